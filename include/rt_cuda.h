@@ -43,6 +43,7 @@ extern "C" {
 /* ---- weight formats (values are GGUF tensor type ids, src/gguf_loader.rs:40-61;
  *      BF16 is GGUF type 30) ------------------------------------------- */
 #define RT_FMT_F32 0
+#define RT_FMT_F16 1 /* paged caches only */
 #define RT_FMT_Q4_0 2
 #define RT_FMT_Q4K 12
 #define RT_FMT_Q6K 14
@@ -430,6 +431,132 @@ int rt_qwen35_reset(rt_qwen35* eng);
 int rt_qwen35_step(rt_qwen35* eng, int32_t token, int32_t position, float* logits);
 /* The device address of the last step's logits ([vocab_size] f32). */
 int rt_qwen35_logits_device(rt_qwen35* eng, const float** out);
+
+/* ---- paged key-value cache ---------------------------------------------
+ * Operators over one layer's cache held in pages, for serving loops whose
+ * sequences grow and shrink (no counterpart in the reference, whose caches
+ * are one contiguous array per layer: Gemma3LayerKvCache,
+ * src/transformer4.rs:1794-1864).  The caller owns every buffer and all of
+ * them are device memory of the context's device.  Calls only enqueue work,
+ * on `stream` (a cudaStream_t; NULL: the context's stream).
+ *
+ * Pools: key and value row (page p, head h, slot s) is head_dim consecutive
+ * elements at p * page_stride + h * head_stride + s * slot_stride (elements;
+ * the same strides for k and v).  Position j of sequence b is slot
+ * j % page_size of page page_table[b * table_stride + j / page_size].
+ * lens[b] counts the cached positions of sequence b, those of the call's new
+ * tokens included.  lens and page_table are read on the device: lengths are
+ * clamped to [0, table_width * page_size]; a page number outside
+ * [0, num_pages) is never followed (reads see zeros, writes are dropped),
+ * and entries that hold no visible position are never followed either, so
+ * freed pages may stay in the table.
+ *
+ * Limits: fmt RT_FMT_F32, RT_FMT_F16 or RT_FMT_BF16; head_dim 64, 128 or 256;
+ * page_size a power of two in 8..256; pools, queries, outputs and rows
+ * 16-byte aligned, all their strides multiples of 16 bytes.
+ *
+ * Workspace: the context keeps one fixed workspace per stream, made by the
+ * first attention or eviction call on that stream (make that call before a
+ * capture: during one it returns RT_E_STATE).  It lives until rt_destroy;
+ * a graph that captured such calls uses it too, so a replay must not overlap
+ * other calls made on the stream it was captured from. */
+typedef struct {
+    void *k, *v;                                   /* pools */
+    int64_t page_stride, head_stride, slot_stride; /* elements */
+    int64_t num_pages;
+    int32_t fmt, kv_heads, head_dim, page_size;
+    const int32_t* page_table;                     /* [num_seqs][table_stride] */
+    int64_t table_stride;
+    int32_t table_width;                           /* entries of a row that may be read */
+    int32_t num_seqs;
+    const int32_t* lens;                           /* [num_seqs] */
+} rt_paged_kv;
+
+/* New key and value rows into the cache.  Row r (of `rows`) holds kv_heads
+ * heads of head_dim elements of src_fmt (f32, f16 or bf16) at
+ * r * row_stride + h * head_stride, rounded to the cache's type (nearest
+ * even; as a plain conversion does, f32 values beyond f16's range become
+ * infinite).  q_start NULL: row b is the last position of sequence b (rows ==
+ * num_seqs).  Otherwise rows q_start[b] .. q_start[b + 1] - 1 (device,
+ * [num_seqs + 1], non-decreasing) are the last positions of sequence b in
+ * order.  Rows before position 0 are dropped. */
+typedef struct {
+    const void *k, *v;
+    int64_t row_stride, head_stride; /* elements of src_fmt */
+    int64_t rows;
+    int32_t src_fmt;
+    const int32_t* q_start;
+} rt_paged_rows;
+int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_rows* rows, void* stream);
+
+/* Attention of new tokens over the paged cache.  Query row r has num_heads
+ * heads (a multiple of kv_heads, at most 16 per KV head; head h reads KV head
+ * h / (num_heads / kv_heads)) in the cache's type.  A token at position t
+ * sees the cached positions j <= t that are within the window (window == 0, or
+ * j > t - window) or among the first `sinks`.
+ *   out[r][h] = sum_j softmax_j(scale * q . k_j) v_j   (cache's type)
+ *   lse[r][h] = log sum_j exp(scale * q . k_j)          (f32; NULL: not wanted)
+ * A token that sees nothing (an empty sequence) gets out 0 and lse -inf.
+ * mass (NULL: not wanted): f32 [num_seqs][kv_heads][>= mass_cap], strides in
+ * elements; mass[b][h][j] += the attention weight of position j summed over
+ * the call's tokens of sequence b and the query heads of KV head h, for every
+ * visible j < mass_cap: the running total that rt_paged_evict ranks by.
+ * Results do not depend on launch order: every sum has a fixed order.
+ *
+ * rt_paged_decode: one token per sequence, at its last position; q_start must
+ * be NULL and rows == num_seqs.  rt_paged_prompt: rows q_start[b] ..
+ * q_start[b + 1] - 1 are the last tokens of sequence b; max_new bounds every
+ * sequence's count (tokens beyond it are not computed).
+ * scratch: rt_paged_scratch bytes of device memory, 256-byte aligned (NULL
+ * when that is 0), which the call's work uses until it has run. */
+typedef struct {
+    const void* q;
+    void* out;
+    int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride; /* elements */
+    float* lse;             /* [rows][lse_row_stride >= num_heads] */
+    int64_t lse_row_stride;
+    int64_t rows;
+    int32_t num_heads;
+    int32_t window, sinks;
+    int32_t max_new;        /* rt_paged_prompt only */
+    float scale;            /* finite, > 0 */
+    int32_t mass_cap;
+    const int32_t* q_start;
+    float* mass;
+    int64_t mass_seq_stride, mass_head_stride;
+    void* scratch;
+    uint64_t scratch_bytes;
+} rt_paged_attn;
+/* Scratch bytes of a call with these arguments (its pointers are not read;
+ * mass only for whether it is NULL). */
+int rt_paged_scratch(const rt_paged_kv* kv, const rt_paged_attn* a, int32_t prompt, uint64_t* bytes);
+int rt_paged_decode(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_attn* a, void* stream);
+int rt_paged_prompt(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_attn* a, void* stream);
+
+/* Trim every sequence to `budget` positions, each KV head on its own: the
+ * first `sinks` positions, the last `recent` ones, and of the others those of
+ * the largest mass (equal ones: the lower position first; NaN counts as
+ * -inf) are copied, in order, to the pages of dst_table ([num_seqs]
+ * [dst_stride], at least ceil(budget / page_size) entries a row), which must
+ * hold no page that a sequence of the call still uses.  Sequences of at most
+ * `budget` positions are copied whole.  sinks + recent <= budget.
+ * kept[b][h][i] (i < budget; contiguous) receives the kept positions in
+ * order, then -1; new_lens[b] = min(lens[b], budget); mass_out (strides of
+ * mass; must not overlap it; mass_cap values a row) receives the kept
+ * positions' mass, then zeros.  mass_cap must cover every length: positions
+ * at mass_cap or beyond count as -inf. */
+typedef struct {
+    const float* mass;
+    float* mass_out;
+    int64_t mass_seq_stride, mass_head_stride;
+    int32_t mass_cap;
+    int32_t budget, sinks, recent;
+    const int32_t* dst_table;
+    int64_t dst_stride;
+    int32_t* kept;
+    int32_t* new_lens;
+} rt_paged_evict_args;
+int rt_paged_evict(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_evict_args* e, void* stream);
 
 /* ---- synthetic inputs ---------------------------------------------------
  * Deterministic, counter-based (SplitMix64) generators for benchmarks and

@@ -24,6 +24,7 @@ RT_E_STATE = -7
 RT_E_TIMEOUT = -8
 
 RT_FMT_F32 = 0
+RT_FMT_F16 = 1
 RT_FMT_Q4_0 = 2
 RT_FMT_Q4K = 12
 RT_FMT_Q6K = 14
@@ -79,6 +80,38 @@ class RtQwen35Layer(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("gate", "up", "down", "input_norm", "post_attn_norm", "in_qkv", "in_z",
                                                "in_a", "in_b", "out_proj", "conv1d_weight", "a_log", "dt_bias",
                                                "norm_weight", "q", "k", "v", "o", "q_norm", "k_norm")]
+
+
+class RtPagedKv(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("page_stride", "head_stride", "slot_stride", "num_pages")] + \
+               [(n, ctypes.c_int32) for n in ("fmt", "kv_heads", "head_dim", "page_size")] + \
+               [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32),
+                ("num_seqs", ctypes.c_int32), ("lens", ctypes.c_void_p)]
+
+
+class RtPagedRows(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("row_stride", "head_stride", "rows")] + \
+               [("src_fmt", ctypes.c_int32), ("q_start", ctypes.c_void_p)]
+
+
+class RtPagedAttn(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("q_row_stride", "q_head_stride", "out_row_stride", "out_head_stride")] + \
+               [("lse", ctypes.c_void_p), ("lse_row_stride", ctypes.c_int64), ("rows", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("num_heads", "window", "sinks", "max_new")] + \
+               [("scale", ctypes.c_float), ("mass_cap", ctypes.c_int32), ("q_start", ctypes.c_void_p),
+                ("mass", ctypes.c_void_p), ("mass_seq_stride", ctypes.c_int64), ("mass_head_stride", ctypes.c_int64),
+                ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_uint64)]
+
+
+class RtPagedEvict(ctypes.Structure):
+    _fields_ = [("mass", ctypes.c_void_p), ("mass_out", ctypes.c_void_p), ("mass_seq_stride", ctypes.c_int64),
+                ("mass_head_stride", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("mass_cap", "budget", "sinks", "recent")] + \
+               [("dst_table", ctypes.c_void_p), ("dst_stride", ctypes.c_int64), ("kept", ctypes.c_void_p),
+                ("new_lens", ctypes.c_void_p)]
 
 
 _vp = ctypes.c_void_p
@@ -141,6 +174,11 @@ SIGNATURES = {
     "rt_decoder_memory": (ctypes.c_int, [_vp, ctypes.POINTER(_u64)]),
     "rt_decoder_launches_per_step": (ctypes.c_int, [_vp, ctypes.POINTER(_i32)]),
     "rt_decoder_read_activation": (ctypes.c_int, [_vp, _i32, _vp, _i64]),
+    "rt_paged_append": (ctypes.c_int, [_vp, _vp, _vp, _vp]),
+    "rt_paged_scratch": (ctypes.c_int, [_vp, _vp, _i32, ctypes.POINTER(_u64)]),
+    "rt_paged_decode": (ctypes.c_int, [_vp, _vp, _vp, _vp]),
+    "rt_paged_prompt": (ctypes.c_int, [_vp, _vp, _vp, _vp]),
+    "rt_paged_evict": (ctypes.c_int, [_vp, _vp, _vp, _vp]),
     "rt_synth_q4k": (None, [_u64, _u64, _i64, _i64, _vp]),
     "rt_nccl_unique_id": (ctypes.c_int, [_vp]),
     "rt_tp_create": (ctypes.c_int, [_vp, _vp, _i32, _i32, _i32, _i32, ctypes.POINTER(_vp)]),

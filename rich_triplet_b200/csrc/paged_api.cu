@@ -1,0 +1,202 @@
+// paged_api.cu -- C ABI of the paged key-value cache (rt_paged_*,
+// include/rt_cuda.h): argument checks, then the launchers of paged.cuh.
+#include <math.h>
+
+#include "paged.cuh"
+#include "rt_internal.h"
+
+using rt::fail;
+
+namespace {
+
+// The context's device is current while a call runs, and the caller's again after it.
+struct DeviceScope {
+    int before = -1;
+    cudaError_t e;
+    explicit DeviceScope(int device) {
+        e = cudaGetDevice(&before);
+        if (e == cudaSuccess && before != device) e = cudaSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+int paged_type(int fmt) {
+    switch (fmt) {
+        case RT_FMT_F32: return rt::kPagedF32;
+        case RT_FMT_F16: return rt::kPagedF16;
+        case RT_FMT_BF16: return rt::kPagedBF16;
+        default: return -1;
+    }
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Every stride a multiple of 16 bytes (and, for the strides of distinct rows, not negative).
+template <typename... S>
+bool strides_ok(int esize, S... s) {
+    return ((s >= 0 && s * esize % 16 == 0) && ...);
+}
+
+int make_kv(rt_ctx* ctx, const char* who, const rt_paged_kv* in, rt::PagedKv* out) {
+    const int type = paged_type(in->fmt);
+    if (type < 0) return fail(ctx, RT_E_FORMAT, "%s: cache format %d is not f32, f16 or bf16", who, in->fmt);
+    if (in->head_dim != 64 && in->head_dim != 128 && in->head_dim != 256)
+        return fail(ctx, RT_E_SHAPE, "%s: head_dim %d is not 64, 128 or 256", who, in->head_dim);
+    if (in->page_size < 8 || in->page_size > 256 || (in->page_size & (in->page_size - 1)))
+        return fail(ctx, RT_E_SHAPE, "%s: page_size %d is not a power of two in 8..256", who, in->page_size);
+    if (in->kv_heads < 1 || in->kv_heads > 65535)
+        return fail(ctx, RT_E_SHAPE, "%s: kv_heads %d out of range", who, in->kv_heads);
+    if (in->num_pages < 0 || in->num_pages > INT32_MAX)
+        return fail(ctx, RT_E_SHAPE, "%s: num_pages %lld out of range", who, static_cast<long long>(in->num_pages));
+    if (in->num_seqs < 0 || in->num_seqs > 65535)
+        return fail(ctx, RT_E_SHAPE, "%s: num_seqs %d out of range (0..65535)", who, in->num_seqs);
+    if (in->table_width < 0 || in->table_stride < in->table_width ||
+        static_cast<int64_t>(in->table_width) * in->page_size > INT32_MAX - 256)
+        return fail(ctx, RT_E_SHAPE, "%s: page table of width %d, row stride %lld", who, in->table_width,
+                    static_cast<long long>(in->table_stride));
+    const int esize = type == rt::kPagedF32 ? 4 : 2;
+    if (!strides_ok(esize, in->page_stride, in->head_stride, in->slot_stride))
+        return fail(ctx, RT_E_INVAL, "%s: cache strides must be multiples of 16 bytes", who);
+    if (in->num_seqs > 0) {
+        if (!in->k || !in->v || !in->lens || (in->table_width > 0 && !in->page_table))
+            return fail(ctx, RT_E_INVAL, "%s: null cache pointer", who);
+        if (!aligned(in->k) || !aligned(in->v)) return fail(ctx, RT_E_INVAL, "%s: the pools must be 16-byte aligned", who);
+    }
+    int lg = 3;
+    while ((1 << lg) < in->page_size) ++lg;
+    *out = rt::PagedKv{in->k,          in->v,           in->page_stride, in->head_stride, in->slot_stride,
+                       in->num_pages,  in->page_table,  in->table_stride, in->lens,       in->table_width,
+                       in->num_seqs,   in->kv_heads,    in->head_dim,    lg,              type};
+    return RT_OK;
+}
+
+int make_attn(rt_ctx* ctx, const char* who, const rt_paged_kv* kv, const rt_paged_attn* in, bool prompt,
+              rt::PagedAttn* out) {
+    const int esize = kv->fmt == RT_FMT_F32 ? 4 : 2;
+    if (in->num_heads < 1 || in->num_heads % kv->kv_heads || in->num_heads / kv->kv_heads > rt::kPagedMaxGroup)
+        return fail(ctx, RT_E_SHAPE, "%s: %d query heads over %d KV heads (a multiple, at most %d each)", who,
+                    in->num_heads, kv->kv_heads, rt::kPagedMaxGroup);
+    if (!(in->scale > 0.f) || !isfinite(in->scale)) return fail(ctx, RT_E_INVAL, "%s: scale must be finite and > 0", who);
+    if (in->window < 0 || in->sinks < 0) return fail(ctx, RT_E_INVAL, "%s: negative window or sinks", who);
+    if (in->rows < 0 || in->rows > INT32_MAX)
+        return fail(ctx, RT_E_SHAPE, "%s: rows %lld out of range", who, static_cast<long long>(in->rows));
+    if (prompt) {
+        if (in->max_new < 0) return fail(ctx, RT_E_INVAL, "%s: negative max_new", who);
+        if (in->rows > 0 && !in->q_start) return fail(ctx, RT_E_INVAL, "%s: null q_start", who);
+    } else {
+        if (in->q_start) return fail(ctx, RT_E_INVAL, "%s: q_start belongs to rt_paged_prompt", who);
+        if (in->rows != kv->num_seqs)
+            return fail(ctx, RT_E_SHAPE, "%s: %lld rows for %d sequences", who, static_cast<long long>(in->rows), kv->num_seqs);
+    }
+    if (in->rows > 0 && (!in->q || !in->out)) return fail(ctx, RT_E_INVAL, "%s: null q or out", who);
+    if (!aligned(in->q) || !aligned(in->out) ||
+        !strides_ok(esize, in->q_row_stride, in->q_head_stride, in->out_row_stride, in->out_head_stride))
+        return fail(ctx, RT_E_INVAL, "%s: q and out must be 16-byte aligned with strides in multiples of 16 bytes", who);
+    if (in->lse && in->lse_row_stride < in->num_heads) return fail(ctx, RT_E_SHAPE, "%s: lse rows overlap", who);
+    if (in->mass && (in->mass_cap < 0 || in->mass_seq_stride < 0 || in->mass_head_stride < 0))
+        return fail(ctx, RT_E_SHAPE, "%s: negative mass size or stride", who);
+    *out = rt::PagedAttn{in->q, in->out, in->q_row_stride, in->q_head_stride, in->out_row_stride, in->out_head_stride,
+                         in->lse, in->lse_row_stride, in->rows, in->num_heads, in->num_heads / kv->kv_heads,
+                         in->window, in->sinks, in->max_new, in->scale, in->mass_cap, prompt ? in->q_start : nullptr,
+                         in->mass, in->mass_seq_stride, in->mass_head_stride, nullptr};
+    return RT_OK;
+}
+
+// The mass pass reads every row's lse: room for it when the caller takes none.
+uint64_t scratch_need(const rt_paged_attn* a) {
+    return a->mass && !a->lse ? (static_cast<uint64_t>(a->rows) * a->num_heads * 4 + 255) / 256 * 256 : 0;
+}
+
+int attend(rt_ctx* ctx, const char* who, const rt_paged_kv* in, const rt_paged_attn* at, bool prompt, void* stream) {
+    if (!ctx || !in || !at) return fail(ctx, RT_E_INVAL, "%s: null argument", who);
+    rt::PagedKv kv;
+    rt::PagedAttn a;
+    if (int rc = make_kv(ctx, who, in, &kv); rc != RT_OK) return rc;
+    if (int rc = make_attn(ctx, who, in, at, prompt, &a); rc != RT_OK) return rc;
+    const uint64_t need = scratch_need(at);
+    if (need > at->scratch_bytes || (need && (!at->scratch || (reinterpret_cast<uintptr_t>(at->scratch) & 255))))
+        return fail(ctx, RT_E_INVAL, "%s: needs %llu bytes of 256-byte aligned scratch", who,
+                    static_cast<unsigned long long>(need));
+    if (a.rows == 0 || kv.nseq == 0 || (prompt && a.max_new == 0)) return RT_OK;
+    DeviceScope scope(ctx->device);
+    RT_CHECK_CUDA(ctx, scope.e);
+    cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
+    a.err = ctx->d_err;
+    if (a.mass && !a.lse) {
+        a.lse = static_cast<float*>(at->scratch);
+        a.lse_row = a.nq;
+    }
+    RT_CHECK_CUDA(ctx, rt::paged_attend_launch(kv, a, s));
+    if (a.mass) RT_CHECK_CUDA(ctx, rt::paged_mass_launch(kv, a, s));
+    return RT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* in, const rt_paged_rows* r, void* stream) {
+    const char* who = "rt_paged_append";
+    if (!ctx || !in || !r) return fail(ctx, RT_E_INVAL, "%s: null argument", who);
+    rt::PagedKv kv;
+    if (int rc = make_kv(ctx, who, in, &kv); rc != RT_OK) return rc;
+    const int st = paged_type(r->src_fmt);
+    if (st < 0) return fail(ctx, RT_E_FORMAT, "%s: row format %d is not f32, f16 or bf16", who, r->src_fmt);
+    if (r->rows < 0 || r->rows > INT32_MAX)
+        return fail(ctx, RT_E_SHAPE, "%s: rows %lld out of range", who, static_cast<long long>(r->rows));
+    if (!r->q_start && r->rows != in->num_seqs)
+        return fail(ctx, RT_E_SHAPE, "%s: %lld rows for %d sequences", who, static_cast<long long>(r->rows), in->num_seqs);
+    if (r->rows == 0 || in->num_seqs == 0) return RT_OK;
+    if (!r->k || !r->v) return fail(ctx, RT_E_INVAL, "%s: null rows", who);
+    if (!aligned(r->k) || !aligned(r->v) || !strides_ok(st == rt::kPagedF32 ? 4 : 2, r->row_stride, r->head_stride))
+        return fail(ctx, RT_E_INVAL, "%s: rows must be 16-byte aligned with strides in multiples of 16 bytes", who);
+    DeviceScope scope(ctx->device);
+    RT_CHECK_CUDA(ctx, scope.e);
+    const rt::PagedRows a{r->k, r->v, r->row_stride, r->head_stride, r->rows, st, r->q_start};
+    RT_CHECK_CUDA(ctx, rt::paged_append_launch(kv, a, stream ? static_cast<cudaStream_t>(stream) : ctx->stream));
+    return RT_OK;
+}
+
+int rt_paged_scratch(const rt_paged_kv* kv, const rt_paged_attn* a, int32_t prompt, uint64_t* bytes) {
+    (void)prompt;
+    if (!kv || !a || !bytes) return RT_E_INVAL;
+    if (kv->kv_heads < 1 || a->num_heads < 1 || a->rows < 0 || kv->num_seqs < 0 || kv->table_width < 0) return RT_E_SHAPE;
+    *bytes = scratch_need(a);
+    return RT_OK;
+}
+
+int rt_paged_decode(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_attn* a, void* stream) {
+    return attend(ctx, "rt_paged_decode", kv, a, false, stream);
+}
+
+int rt_paged_prompt(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_attn* a, void* stream) {
+    return attend(ctx, "rt_paged_prompt", kv, a, true, stream);
+}
+
+int rt_paged_evict(rt_ctx* ctx, const rt_paged_kv* in, const rt_paged_evict_args* e, void* stream) {
+    const char* who = "rt_paged_evict";
+    if (!ctx || !in || !e) return fail(ctx, RT_E_INVAL, "%s: null argument", who);
+    rt::PagedKv kv;
+    if (int rc = make_kv(ctx, who, in, &kv); rc != RT_OK) return rc;
+    if (e->budget < 1 || e->sinks < 0 || e->recent < 0 || static_cast<int64_t>(e->sinks) + e->recent > e->budget)
+        return fail(ctx, RT_E_INVAL, "%s: sinks %d + recent %d must lie in 0..budget %d", who, e->sinks, e->recent, e->budget);
+    if (e->mass_cap < 0 || e->mass_seq_stride < 0 || e->mass_head_stride < 0)
+        return fail(ctx, RT_E_SHAPE, "%s: negative mass size or stride", who);
+    if (e->dst_stride < (static_cast<int64_t>(e->budget) + in->page_size - 1) / in->page_size)
+        return fail(ctx, RT_E_SHAPE, "%s: %lld destination pages a row hold fewer than %d positions", who,
+                    static_cast<long long>(e->dst_stride), e->budget);
+    if (in->num_seqs == 0) return RT_OK;
+    if (!e->mass || !e->mass_out || !e->dst_table || !e->kept || !e->new_lens)
+        return fail(ctx, RT_E_INVAL, "%s: null argument", who);
+    DeviceScope scope(ctx->device);
+    RT_CHECK_CUDA(ctx, scope.e);
+    const rt::PagedEvict a{e->mass, e->mass_out, e->mass_seq_stride, e->mass_head_stride, e->mass_cap, e->budget,
+                           e->sinks, e->recent, e->dst_table, e->dst_stride, e->kept, e->new_lens};
+    RT_CHECK_CUDA(ctx, rt::paged_evict_launch(kv, a, stream ? static_cast<cudaStream_t>(stream) : ctx->stream));
+    return RT_OK;
+}
+
+}  // extern "C"
