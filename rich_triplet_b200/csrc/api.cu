@@ -107,6 +107,7 @@ void rt_destroy(rt_ctx* ctx) {
     cudaFree(ctx->io);
     cudaFree(ctx->gemv_part);
     cudaFree(ctx->gemv_cnt);
+    for (auto& w : ctx->paged_ws) cudaFree(w.second);
     cudaFree(ctx->d_err);
     if (ctx->stream) cudaStreamDestroy(ctx->stream);
     delete ctx;

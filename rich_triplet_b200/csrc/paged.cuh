@@ -105,8 +105,14 @@ __device__ __forceinline__ int row_seq(const int32_t* q_start, int nseq, int64_t
 }
 
 cudaError_t paged_append_launch(const PagedKv& kv, const PagedRows& r, cudaStream_t s);
-cudaError_t paged_attend_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s);
-cudaError_t paged_mass_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s);
+// Fixed workspace of a stream: counters (zero before its first call; every
+// call leaves them zero), then partial results.
+size_t paged_workspace_bytes(int num_sms);
+size_t paged_counter_bytes(int num_sms);
+size_t paged_decode_scratch(const PagedKv& kv, const PagedAttn& a);
+cudaError_t paged_decode_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, void* scratch, int num_sms,
+                                cudaStream_t s);
+cudaError_t paged_prompt_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s);
 cudaError_t paged_evict_launch(const PagedKv& kv, const PagedEvict& e, cudaStream_t s);
 
 template <typename T>

@@ -105,9 +105,33 @@ int make_attn(rt_ctx* ctx, const char* who, const rt_paged_kv* kv, const rt_page
     return RT_OK;
 }
 
-// The mass pass reads every row's lse: room for it when the caller takes none.
-uint64_t scratch_need(const rt_paged_attn* a) {
-    return a->mass && !a->lse ? (static_cast<uint64_t>(a->rows) * a->num_heads * 4 + 255) / 256 * 256 : 0;
+// The prompt mass pass reads every row's lse: room for it when the caller takes none.
+uint64_t scratch_need(const rt::PagedKv& kv, const rt::PagedAttn& a, bool prompt) {
+    if (!prompt) return rt::paged_decode_scratch(kv, a);
+    return a.mass && !a.lse ? (static_cast<uint64_t>(a.rows) * a.nq * 4 + 255) / 256 * 256 : 0;
+}
+
+// The stream's workspace, made on first use.
+int workspace(rt_ctx* ctx, const char* who, cudaStream_t s, void** out) {
+    auto it = ctx->paged_ws.find(s);
+    if (it != ctx->paged_ws.end()) {
+        *out = it->second;
+        return RT_OK;
+    }
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    RT_CHECK_CUDA(ctx, cudaStreamIsCapturing(s, &st));
+    if (st != cudaStreamCaptureStatusNone)
+        return fail(ctx, RT_E_STATE, "%s: the stream's workspace does not exist yet; make one call before the capture", who);
+    void* p = nullptr;
+    if (int rc = rt::dev_alloc(ctx, &p, rt::paged_workspace_bytes(ctx->num_sms), "paged workspace"); rc != RT_OK) return rc;
+    const cudaError_t e = cudaMemsetAsync(p, 0, rt::paged_counter_bytes(ctx->num_sms), s);
+    if (e != cudaSuccess) {
+        cudaFree(p);
+        return fail(ctx, RT_E_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    }
+    ctx->paged_ws[s] = p;
+    *out = p;
+    return RT_OK;
 }
 
 int attend(rt_ctx* ctx, const char* who, const rt_paged_kv* in, const rt_paged_attn* at, bool prompt, void* stream) {
@@ -116,7 +140,7 @@ int attend(rt_ctx* ctx, const char* who, const rt_paged_kv* in, const rt_paged_a
     rt::PagedAttn a;
     if (int rc = make_kv(ctx, who, in, &kv); rc != RT_OK) return rc;
     if (int rc = make_attn(ctx, who, in, at, prompt, &a); rc != RT_OK) return rc;
-    const uint64_t need = scratch_need(at);
+    const uint64_t need = scratch_need(kv, a, prompt);
     if (need > at->scratch_bytes || (need && (!at->scratch || (reinterpret_cast<uintptr_t>(at->scratch) & 255))))
         return fail(ctx, RT_E_INVAL, "%s: needs %llu bytes of 256-byte aligned scratch", who,
                     static_cast<unsigned long long>(need));
@@ -125,12 +149,17 @@ int attend(rt_ctx* ctx, const char* who, const rt_paged_kv* in, const rt_paged_a
     RT_CHECK_CUDA(ctx, scope.e);
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     a.err = ctx->d_err;
-    if (a.mass && !a.lse) {
-        a.lse = static_cast<float*>(at->scratch);
-        a.lse_row = a.nq;
+    if (prompt) {
+        if (a.mass && !a.lse) {
+            a.lse = static_cast<float*>(at->scratch);
+            a.lse_row = a.nq;
+        }
+        RT_CHECK_CUDA(ctx, rt::paged_prompt_launch(kv, a, s));
+    } else {
+        void* ws = nullptr;
+        if (int rc = workspace(ctx, who, s, &ws); rc != RT_OK) return rc;
+        RT_CHECK_CUDA(ctx, rt::paged_decode_launch(kv, a, ws, at->scratch, ctx->num_sms, s));
     }
-    RT_CHECK_CUDA(ctx, rt::paged_attend_launch(kv, a, s));
-    if (a.mass) RT_CHECK_CUDA(ctx, rt::paged_mass_launch(kv, a, s));
     return RT_OK;
 }
 
@@ -160,11 +189,18 @@ int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* in, const rt_paged_rows* r, 
     return RT_OK;
 }
 
-int rt_paged_scratch(const rt_paged_kv* kv, const rt_paged_attn* a, int32_t prompt, uint64_t* bytes) {
-    (void)prompt;
-    if (!kv || !a || !bytes) return RT_E_INVAL;
-    if (kv->kv_heads < 1 || a->num_heads < 1 || a->rows < 0 || kv->num_seqs < 0 || kv->table_width < 0) return RT_E_SHAPE;
-    *bytes = scratch_need(a);
+int rt_paged_scratch(const rt_paged_kv* in, const rt_paged_attn* at, int32_t prompt, uint64_t* bytes) {
+    if (!in || !at || !bytes) return RT_E_INVAL;
+    if (in->page_size < 1 || at->rows < 0 || in->table_width < 0 || at->num_heads < 1) return RT_E_SHAPE;
+    rt::PagedKv kv = {};
+    rt::PagedAttn a = {};
+    kv.width = in->table_width;
+    while ((1 << kv.page_log2) < in->page_size) ++kv.page_log2;
+    a.rows = at->rows;
+    a.nq = at->num_heads;
+    a.mass = at->mass;
+    a.lse = at->lse;
+    *bytes = scratch_need(kv, a, prompt != 0);
     return RT_OK;
 }
 

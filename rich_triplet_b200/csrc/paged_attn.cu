@@ -1,4 +1,5 @@
-// paged_attn.cu -- attention over a paged cache.
+// paged_attn.cu -- attention of several new tokens per sequence over a paged
+// cache (rt_paged_prompt).
 //
 // One warp per (query row, head): lane l holds the dims l, l + 32, ... of the
 // query and of the output, and walks the visible positions with a running
@@ -14,11 +15,6 @@ namespace {
 
 // Row r's sequence and the positions its token sees (n of them up to and with itself).
 __device__ __forceinline__ bool row_token(const PagedKv& kv, const PagedAttn& a, int64_t r, int& b, int& n) {
-    if (!a.q_start) {
-        b = static_cast<int>(r);
-        n = kv.len(b);
-        return true;
-    }
     b = row_seq(a.q_start, kv.nseq, r);
     const int64_t first = a.q_start[b], count = a.q_start[b + 1] - first, i = r - first;
     if (i < 0 || i >= count || i >= a.max_new) return false;
@@ -77,9 +73,8 @@ __global__ void __launch_bounds__(128) paged_mass_kernel(const PagedKv kv, const
     const int j = blockIdx.x * 4 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
     const int len = kv.len(b);
     if (j >= len || j >= a.mass_cap) return;
-    const int64_t first = a.q_start ? a.q_start[b] : b;
-    const int64_t all = a.q_start ? a.q_start[b + 1] - first : 1;
-    const int64_t count = a.q_start && all > a.max_new ? a.max_new : all;
+    const int64_t first = a.q_start[b], all = a.q_start[b + 1] - first;
+    const int64_t count = all > a.max_new ? a.max_new : all;
     const int64_t t0 = len - all;  // position of the first new token
     const int64_t off = kv.row(b, j);
     float k[E];
@@ -125,12 +120,10 @@ cudaError_t mass(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t paged_attend_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
-    return kv.type == kPagedF32 ? attend<float>(kv, a, s)
-         : kv.type == kPagedF16 ? attend<__half>(kv, a, s) : attend<__nv_bfloat16>(kv, a, s);
-}
-
-cudaError_t paged_mass_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
+cudaError_t paged_prompt_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
+    cudaError_t e = kv.type == kPagedF32 ? attend<float>(kv, a, s)
+                  : kv.type == kPagedF16 ? attend<__half>(kv, a, s) : attend<__nv_bfloat16>(kv, a, s);
+    if (e != cudaSuccess || !a.mass) return e;
     return kv.type == kPagedF32 ? mass<float>(kv, a, s)
          : kv.type == kPagedF16 ? mass<__half>(kv, a, s) : mass<__nv_bfloat16>(kv, a, s);
 }
