@@ -112,7 +112,9 @@ size_t paged_counter_bytes(int num_sms);
 size_t paged_decode_scratch(const PagedKv& kv, const PagedAttn& a);
 cudaError_t paged_decode_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, void* scratch, int num_sms,
                                 cudaStream_t s);
-cudaError_t paged_prompt_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s);
+size_t paged_prompt_part_bytes(int num_sms);
+cudaError_t paged_prompt16_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s);
+cudaError_t paged_prompt_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s);
 cudaError_t paged_evict_launch(const PagedKv& kv, const PagedEvict& e, cudaStream_t s);
 
 template <typename T>

@@ -34,7 +34,7 @@ int paged_type(int fmt) {
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Every stride a multiple of 16 bytes (and, for the strides of distinct rows, not negative).
+// Every stride a multiple of 16 bytes and not negative.
 template <typename... S>
 bool strides_ok(int esize, S... s) {
     return ((s >= 0 && s * esize % 16 == 0) && ...);
@@ -49,7 +49,7 @@ int make_kv(rt_ctx* ctx, const char* who, const rt_paged_kv* in, rt::PagedKv* ou
         return fail(ctx, RT_E_SHAPE, "%s: page_size %d is not a power of two in 8..256", who, in->page_size);
     if (in->kv_heads < 1 || in->kv_heads > 65535)
         return fail(ctx, RT_E_SHAPE, "%s: kv_heads %d out of range", who, in->kv_heads);
-    if (in->num_pages < 0 || in->num_pages > INT32_MAX)
+    if (in->num_pages < 1 || in->num_pages > INT32_MAX - 1)
         return fail(ctx, RT_E_SHAPE, "%s: num_pages %lld out of range", who, static_cast<long long>(in->num_pages));
     if (in->num_seqs < 0 || in->num_seqs > 65535)
         return fail(ctx, RT_E_SHAPE, "%s: num_seqs %d out of range (0..65535)", who, in->num_seqs);
@@ -60,6 +60,9 @@ int make_kv(rt_ctx* ctx, const char* who, const rt_paged_kv* in, rt::PagedKv* ou
     const int esize = type == rt::kPagedF32 ? 4 : 2;
     if (!strides_ok(esize, in->page_stride, in->head_stride, in->slot_stride))
         return fail(ctx, RT_E_INVAL, "%s: cache strides must be multiples of 16 bytes", who);
+    if (in->slot_stride < in->head_dim || (in->kv_heads > 1 && in->head_stride < in->head_dim) ||
+        (in->num_pages > 1 && in->page_stride < in->head_dim))
+        return fail(ctx, RT_E_SHAPE, "%s: the rows of the cache overlap", who);
     if (in->num_seqs > 0) {
         if (!in->k || !in->v || !in->lens || (in->table_width > 0 && !in->page_table))
             return fail(ctx, RT_E_INVAL, "%s: null cache pointer", who);
@@ -149,17 +152,17 @@ int attend(rt_ctx* ctx, const char* who, const rt_paged_kv* in, const rt_paged_a
     RT_CHECK_CUDA(ctx, scope.e);
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     a.err = ctx->d_err;
-    if (prompt) {
-        if (a.mass && !a.lse) {
-            a.lse = static_cast<float*>(at->scratch);
-            a.lse_row = a.nq;
-        }
-        RT_CHECK_CUDA(ctx, rt::paged_prompt_launch(kv, a, s));
-    } else {
-        void* ws = nullptr;
-        if (int rc = workspace(ctx, who, s, &ws); rc != RT_OK) return rc;
+    void* ws = nullptr;
+    if (int rc = workspace(ctx, who, s, &ws); rc != RT_OK) return rc;
+    if (!prompt) {
         RT_CHECK_CUDA(ctx, rt::paged_decode_launch(kv, a, ws, at->scratch, ctx->num_sms, s));
+        return RT_OK;
     }
+    if (a.mass && !a.lse) {
+        a.lse = static_cast<float*>(at->scratch);
+        a.lse_row = a.nq;
+    }
+    RT_CHECK_CUDA(ctx, rt::paged_prompt_launch(kv, a, ws, ctx->num_sms, s));
     return RT_OK;
 }
 

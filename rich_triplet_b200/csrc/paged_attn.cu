@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(128) paged_mass_kernel(const PagedKv kv, const
     const int len = kv.len(b);
     if (j >= len || j >= a.mass_cap) return;
     const int64_t first = a.q_start[b], all = a.q_start[b + 1] - first;
-    const int64_t count = all > a.max_new ? a.max_new : all;
+    const int64_t count = min(min(all, static_cast<int64_t>(a.max_new)), a.rows - first);
     const int64_t t0 = len - all;  // position of the first new token
     const int64_t off = kv.row(b, j);
     float k[E];
@@ -120,9 +120,8 @@ cudaError_t mass(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t paged_prompt_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
-    cudaError_t e = kv.type == kPagedF32 ? attend<float>(kv, a, s)
-                  : kv.type == kPagedF16 ? attend<__half>(kv, a, s) : attend<__nv_bfloat16>(kv, a, s);
+cudaError_t paged_prompt_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s) {
+    cudaError_t e = kv.type == kPagedF32 ? attend<float>(kv, a, s) : paged_prompt16_launch(kv, a, workspace, num_sms, s);
     if (e != cudaSuccess || !a.mass) return e;
     return kv.type == kPagedF32 ? mass<float>(kv, a, s)
          : kv.type == kPagedF16 ? mass<__half>(kv, a, s) : mass<__nv_bfloat16>(kv, a, s);

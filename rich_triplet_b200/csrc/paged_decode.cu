@@ -671,7 +671,8 @@ int decode_grid(int num_sms) { return 2 * (num_sms > 0 ? num_sms : 148); }
 
 size_t paged_workspace_bytes(int num_sms) {
     const size_t grid = decode_grid(num_sms);
-    return paged_counter_bytes(num_sms) + grid * 2 * kPagedMaxGroup * (256 + 4) * sizeof(float);
+    return paged_counter_bytes(num_sms) +
+           std::max(grid * 2 * kPagedMaxGroup * (256 + 4) * sizeof(float), paged_prompt_part_bytes(num_sms));
 }
 
 size_t paged_counter_bytes(int num_sms) { return (decode_grid(num_sms) * sizeof(uint32_t) + 255) / 256 * 256; }

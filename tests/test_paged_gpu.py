@@ -584,3 +584,13 @@ def test_refusals():
     # and after all that the operators still work
     dec(q, *c.args(), **ok)
     torch.cuda.synchronize()
+
+
+def test_prompt_more_row_tiles_than_sms():
+    """Several waves of CTAs over long windowed walks, and again: a wait that is
+    only sometimes late shows here."""
+    for _ in range(3):
+        check_prompt([2600, 900], [2000, 900], 16, 4, 256, 64, F16, window=1024, sinks=4, seed=5)
+        check_prompt([2600, 900], [2000, 900], 16, 4, 128, 64, BF16, seed=6)
+    from rich_triplet_b200 import paged
+    paged._context(torch.device("cuda", torch.cuda.current_device())).sync()  # raises if a wait gave up
