@@ -5,6 +5,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <cuda.h>  // CUtensorMap
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -113,6 +114,8 @@ size_t paged_decode_scratch(const PagedKv& kv, const PagedAttn& a);
 cudaError_t paged_decode_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, void* scratch, int num_sms,
                                 cudaStream_t s);
 size_t paged_prompt_part_bytes(int num_sms);
+bool paged_pool_map(const PagedKv& kv, void* pool, CUtensorMap* out);
+cudaError_t paged_prompt_mass16_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s);
 cudaError_t paged_prompt16_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s);
 cudaError_t paged_prompt_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s);
 cudaError_t paged_evict_launch(const PagedKv& kv, const PagedEvict& e, cudaStream_t s);

@@ -84,7 +84,7 @@ int make_attn(rt_ctx* ctx, const char* who, const rt_paged_kv* kv, const rt_page
                     in->num_heads, kv->kv_heads, rt::kPagedMaxGroup);
     if (!(in->scale > 0.f) || !isfinite(in->scale)) return fail(ctx, RT_E_INVAL, "%s: scale must be finite and > 0", who);
     if (in->window < 0 || in->sinks < 0) return fail(ctx, RT_E_INVAL, "%s: negative window or sinks", who);
-    if (in->rows < 0 || in->rows > INT32_MAX)
+    if (in->rows < 0 || in->rows > INT32_MAX / rt::kPagedMaxGroup)
         return fail(ctx, RT_E_SHAPE, "%s: rows %lld out of range", who, static_cast<long long>(in->rows));
     if (prompt) {
         if (in->max_new < 0) return fail(ctx, RT_E_INVAL, "%s: negative max_new", who);

@@ -1,0 +1,295 @@
+// paged_mass.cu -- attention weights of a prompt summed per cached position
+// (the `mass` of rt_paged_prompt) for 16-bit caches, on the tcgen05 tensor
+// cores.
+//
+// The weight exp(s - lse) needs the row's final log-sum, so this is a second
+// pass over the scores, after the attention: 2 D flops per visible pair and
+// head, one exponential.  It is transposed, S^T = K Q^T, so that a thread owns
+// one position (a tensor-memory lane) and adds the weights of the rows, its
+// columns, in registers, in a fixed order, with no exchange between threads.
+//
+// A CTA takes one tile of 128 positions of a (sequence, KV head), keeps its
+// keys in shared memory and walks the (token, head) rows that see it, 128 at a
+// time: a loading warpgroup gathers the query rows with cp.async into the
+// 128-byte-swizzled ring, the MMA thread forms the scores in one of four
+// tensor-memory buffers, and two warpgroups take alternate tiles.  Tiles of
+// early positions, which most rows see, start first.
+//
+// Waits are bounded as in paged_prompt.cu.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+namespace rt {
+
+namespace {
+
+constexpr int kTile = 128;     // positions, and rows, of a tile
+constexpr int kSumGroups = 2;  // warpgroups that add
+constexpr int kBufs = 4;       // score buffers in tensor memory
+constexpr int kThreads = (kSumGroups * 4 + 4 + 1) * 32;
+
+template <int D>
+struct MCfg {
+    static constexpr int kChunk = kTile * 128;  // 64 columns of 128 rows
+    static constexpr int kOperand = (D / 64) * kChunk;
+    static constexpr int NST = D == 256 ? 2 : 4;
+    static constexpr int kOffRing = kOperand;
+    static constexpr int kOffRow = kOffRing + NST * kOperand;  // [adding warp][128] {log-sum, token position}
+    static constexpr int kOffTotal = kOffRow + kSumGroups * 4 * kTile * 8;  // [128] the second group's totals
+    static constexpr int kOffBar = kOffTotal + kTile * 4;
+    static constexpr int kBars = 2 * NST + 2 * kBufs + 2;
+    static constexpr int kOffMisc = kOffBar + kBars * 8;
+    static constexpr int kSmem = kOffMisc + 16 + 1024;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_prompt_mass_kernel(const __grid_constant__ CUtensorMap tm_k, const PagedKv kv, const PagedAttn a, const float scale2) {
+    using C = MCfg<D>;
+    constexpr int NST = C::NST;
+    constexpr bool BF16 = !std::is_same<T, __half>::value;
+    extern __shared__ uint8_t smem_raw[];
+
+    // ---- the positions of this CTA and the rows that see one of them ----
+    const int G = a.G;
+    const int64_t bhs = static_cast<int64_t>(kv.nseq) * kv.nkv;
+    const int j0 = static_cast<int>(blockIdx.x / bhs) * kTile;
+    const int b = static_cast<int>(blockIdx.x % bhs) / kv.nkv, h = static_cast<int>(blockIdx.x % bhs) % kv.nkv;
+    const int64_t q_first = a.q_start[b];
+    const int all = a.q_start[b + 1] - static_cast<int>(q_first), len = kv.len(b);
+    if (all <= 0 || q_first < 0) return;
+    const int m = static_cast<int>(min(static_cast<int64_t>(min(all, a.max_new)), a.rows - q_first));  // tokens computed
+    const int pos0 = len - all;
+    const int j_end = min(j0 + kTile, min(len, a.mass_cap));  // positions whose total is kept
+    const int i_lo = max(0, j0 - pos0);
+    int i_hi = m - 1;
+    if (a.window > 0 && j0 >= a.sinks)
+        i_hi = static_cast<int>(min(static_cast<int64_t>(i_hi), static_cast<int64_t>(j_end) - 1 + a.window - 1 - pos0));
+    if (j_end <= j0 || i_hi < i_lo) return;
+    const int r_begin = i_lo * G, r_end = (i_hi + 1) * G;  // rows * G fits 32 bits (checked by the caller)
+    const int n = (r_end - r_begin + kTile - 1) / kTile;
+
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
+    uint8_t* ring = sm + C::kOffRing;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + C::kOffBar);
+    uint64_t* empty = full + NST;
+    uint64_t* s_full = empty + NST;
+    uint64_t* s_free = s_full + kBufs;
+    uint64_t* k_full = s_free + kBufs;
+    uint64_t* drain = k_full + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::kOffMisc);
+    volatile int* abort = reinterpret_cast<volatile int*>(sm + C::kOffMisc + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x & 127;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NST; ++s) {
+            mbar_init(&full[s], 4);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < kBufs; ++s) {
+            mbar_init(&s_full[s], 1);
+            mbar_init(&s_free[s], 4);
+        }
+        mbar_init(k_full, 1);
+        mbar_init(drain, 1);
+        *abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 0) tc::alloc(tmem_slot, 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *tmem_slot;
+    float total = 0.f;
+
+    if (warp == kSumGroups * 4 + 4) {
+        // ---- the keys, then the products ----
+        if (lane == 0) mbar_arrive_expect_tx(k_full, C::kOperand);
+        __syncwarp();
+        const int rows = min(1 << kv.page_log2, kTile), boxes = kTile / rows;
+        for (int i = lane; i < boxes * (D / 64); i += 32) {
+            const int chunk = i / boxes, box = i % boxes, p = j0 + box * rows;
+            int page = -1;
+            if (p < len) page = kv.table[b * kv.table_stride + (p >> kv.page_log2)];
+            if (static_cast<uint32_t>(page) >= static_cast<uint64_t>(kv.num_pages)) page = static_cast<int>(kv.num_pages);
+            tc::tma_4d(sm + chunk * C::kChunk + box * rows * 128, &tm_k, 64 * chunk, p & ((1 << kv.page_log2) - 1), h, page,
+                       k_full);
+        }
+        __syncwarp();
+        if (lane == 0) {
+            constexpr uint32_t kId = tc::idesc_f16(BF16, kTile, false);
+            bool ok = tc::wait_phase(k_full, 0u, abort);
+            for (int i = 0; i < n && ok; ++i) {
+                const int s = i % NST, buf = i % kBufs;
+                ok = tc::wait_phase(&full[s], static_cast<uint32_t>(i / NST) & 1u, abort) &&
+                     (i < kBufs || tc::wait_phase(&s_free[buf], static_cast<uint32_t>(i / kBufs - 1) & 1u, abort));
+                if (!ok) break;
+                tc::fence_after();
+                const uint32_t kb = smem_u32(sm), qb = smem_u32(ring + s * C::kOperand);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t at = (k >> 2) * C::kChunk + (k & 3) * 32;
+                    tc::mma_ss(tmem + buf * kTile, tc::desc_sw128(kb + at, 16), tc::desc_sw128(qb + at, 16), kId, k > 0);
+                }
+                tc::commit(&empty[s]);
+                tc::commit(&s_full[buf]);
+            }
+            if (!ok) tc::give_up(abort, a.err);
+            tc::commit(drain);
+            (void)mbar_wait_timed(drain, 0u);
+            (void)mbar_wait_timed(k_full, 0u);
+        }
+        __syncwarp();
+    } else if (warp >= kSumGroups * 4) {
+        // ---- query rows into the ring, one tile ahead of the one that is handed over ----
+        constexpr int CPR = D / 8;
+        bool ok = true;
+        for (int i = 0; i <= n; ++i) {
+            if (i < n) {
+                const int s = i % NST;
+                ok = ok && __all_sync(0xffffffffu, i < NST || tc::wait_phase(&empty[s], static_cast<uint32_t>(i / NST - 1) & 1u, abort));
+                if (!ok) break;
+                const uint32_t dst = smem_u32(ring + s * C::kOperand);
+                const int r0 = r_begin + i * kTile;
+#pragma unroll 8
+                for (int x = tid; x < kTile * CPR; x += 128) {
+                    const int row = x / CPR, ch = x % CPR;
+                    const int rho = min(r0 + row, r_end - 1), tok = rho / G;
+                    const T* src = static_cast<const T*>(a.q) + (q_first + tok) * a.q_row +
+                                   (h * G + rho - tok * G) * a.q_head + ch * 8;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                     dst + (ch >> 3) * C::kChunk + row * 128 + (((ch & 7) ^ (row & 7)) << 4)),
+                                 "l"(src)
+                                 : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (i > 0) {
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[(i - 1) % NST]);
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (!ok) tc::give_up(abort, a.err);
+    } else {
+        // ---- thread = position ----
+        const int grp = warp >> 2, j = j0 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+        // a warp's own copy of the tile's rows: log-sum (powers of two; +inf for
+        // none, whose weight is then 0) and position
+        float2* rb = reinterpret_cast<float2*>(sm + C::kOffRow) + warp * kTile;
+        float2 next[4];
+        auto load_rows = [&](int i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int rho = r_begin + i * kTile + lane + 32 * e, tok = rho / G;
+                next[e] = make_float2(INFINITY, 0.f);
+                if (i >= n || rho >= r_end) continue;
+                const float z = a.lse[(q_first + tok) * a.lse_row + h * G + rho - tok * G];
+                next[e] = make_float2(z == -INFINITY ? INFINITY : z * 1.44269504088896341f, __int_as_float(pos0 + tok));
+            }
+        };
+        load_rows(grp);
+        bool ok = true;
+        for (int i = grp; i < n; i += kSumGroups) {
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rb[lane + 32 * e] = next[e];
+            __syncwarp();
+            load_rows(i + kSumGroups);
+            const int buf = i % kBufs;
+            ok = __all_sync(0xffffffffu, tc::wait_phase(&s_full[buf], static_cast<uint32_t>(i / kBufs) & 1u, abort));
+            if (!ok) break;
+            tc::fence_after();
+            const int r0 = r_begin + i * kTile, r1 = min(r0 + kTile, r_end) - 1;
+            const int t_lo = pos0 + r0 / G, t_hi = pos0 + r1 / G;
+            const bool masked = j0 + kTile - 1 > t_lo || (a.window > 0 && j0 <= t_hi - a.window);
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int c = 0; c < kTile; c += 32) {
+                float x[32];
+                tc::ld32(tmem + lanes + buf * kTile + c, x);
+                tc::wait_ld();
+                tc::tie32(x);
+                if (c == kTile - 32) {
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_free[buf]);
+                }
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int t = __float_as_int(rb[c + e].y);
+                        if (j > t || (a.window > 0 && j <= t - a.window && j >= a.sinks)) x[e] = -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const float4 z = *reinterpret_cast<const float4*>(&rb[c + e]);
+                    part[e & 2] += tc::ex2(fmaf(x[e], scale2, -z.x));
+                    part[(e & 2) + 1] += tc::ex2(fmaf(x[e + 1], scale2, -z.z));
+                }
+            }
+            total += (part[0] + part[1]) + (part[2] + part[3]);
+        }
+        if (!ok) tc::give_up(abort, a.err);
+        if (grp == 1) reinterpret_cast<float*>(sm + C::kOffTotal)[tid] = total;
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp < 4) {
+        const int j = j0 + threadIdx.x;
+        if (j < j_end && !*abort)
+            a.mass[b * a.mass_seq + h * a.mass_head + j] +=
+                total + reinterpret_cast<const float*>(sm + C::kOffTotal)[threadIdx.x];
+    }
+    if (warp == 0) {
+        tc::fence_after();
+        tc::dealloc(tmem, 512);
+    }
+}
+
+template <typename T, int D>
+cudaError_t launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
+    using C = MCfg<D>;
+    auto kernel = paged_prompt_mass_kernel<T, D>;
+    static bool done[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !done[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) done[dev] = true;
+    }
+    CUtensorMap tk;
+    if (!paged_pool_map(kv, kv.k, &tk)) return cudaErrorInvalidValue;
+    const int64_t cap = std::min<int64_t>(static_cast<int64_t>(kv.width) << kv.page_log2, a.mass_cap);
+    const int64_t grid = (cap + kTile - 1) / kTile * kv.nseq * kv.nkv;
+    if (grid == 0) return cudaSuccess;
+    if (grid > INT32_MAX) return cudaErrorInvalidValue;
+    kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmem, s>>>(tk, kv, a, a.scale * 1.44269504088896341f);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t by_dim(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
+    if (kv.D == 64) return launch<T, 64>(kv, a, s);
+    if (kv.D == 128) return launch<T, 128>(kv, a, s);
+    return launch<T, 256>(kv, a, s);
+}
+
+}  // namespace
+
+cudaError_t paged_prompt_mass16_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
+    return kv.type == kPagedF16 ? by_dim<__half>(kv, a, s) : by_dim<__nv_bfloat16>(kv, a, s);
+}
+
+}  // namespace rt

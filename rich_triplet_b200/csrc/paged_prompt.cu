@@ -90,43 +90,6 @@ struct PromptWork {
     float scale2;   // scale * log2(e)
 };
 
-// Wait for phase `parity` of `bar`; gives up after a second or once *abort is set.
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort) {
-    const uint32_t addr = smem_u32(bar);
-    uint64_t t0 = 0;
-    for (uint32_t it = 1;; ++it) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(addr), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((it & 1023u) == 0u) {
-            if (*abort) return false;
-            uint64_t t;
-            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-            if (it == 1024u) t0 = t;
-            else if (t - t0 > 1000000000ull) return false;
-        }
-    }
-}
-
-__device__ __forceinline__ void give_up(volatile int* abort, int* err) {
-    *abort = 1;
-    if (err) atomicExch(err, kErrMbarTimeout);
-}
-
-__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* tm, int x, int slot, int head, int page, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-            smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
-        : "memory");
-}
-
 __device__ __forceinline__ uint32_t pack16(float a, float b, __half) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -135,12 +98,6 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, __nv_bfloat16) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // The key tiles of rows whose tokens stand at t_min .. t_max.
 struct Walk {
     int first_tiles, w_tile, count;  // tiles of the first tokens, then from w_tile on
@@ -270,13 +227,13 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             if (chunk < C::SD / 64 && p < len) page = kv.table[b * kv.table_stride + (p >> kv.page_log2)];
             if (static_cast<uint32_t>(page) >= static_cast<uint64_t>(kv.num_pages)) page = static_cast<int>(kv.num_pages);
             if (lane == 0) {
-                ok = e < NST || wait_phase(&empty[s], static_cast<uint32_t>(e / NST - 1) & 1u, abort);
+                ok = e < NST || tc::wait_phase(&empty[s], static_cast<uint32_t>(e / NST - 1) & 1u, abort);
                 if (ok) mbar_arrive_expect_tx(&full[s], C::kStage);
-                else give_up(abort, a.err);
+                else tc::give_up(abort, a.err);
             }
             ok = __shfl_sync(0xffffffffu, ok, 0);
             if (ok && chunk < C::SD / 64)
-                tma_4d(ring + s * C::kStage + chunk * C::kChunk + box * rows * 128, is_v ? &tm_v : &tm_k, col0 + 64 * chunk,
+                tc::tma_4d(ring + s * C::kStage + chunk * C::kChunk + box * rows * 128, is_v ? &tm_v : &tm_k, col0 + 64 * chunk,
                        p & ((1 << kv.page_log2) - 1), h, page, &full[s]);
             if (ok) ++done;
         }
@@ -292,12 +249,12 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
 #pragma unroll
             for (int t = 0; t < NQ; ++t) nt[t] = tiles_of(t);
             auto last_t = [&](int j) { return NQ == 2 && j < nt[NQ - 1] ? 1 : 0; };
-            bool ok = wait_phase(q_full, 0u, abort);
+            bool ok = tc::wait_phase(q_full, 0u, abort);
             auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
 #pragma unroll
                 for (int sp = 0; sp < SPT; ++sp) {
                     const int e = k_seq(j) + sp, s = e % NST;
-                    ok = ok && wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
+                    ok = ok && tc::wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
                     if (!ok) return;
                     tc::fence_after();
                     const uint32_t kb = smem_u32(ring + s * C::kStage), qb = smem_u32(sm + t * C::kQTile) + sp * C::kStage;
@@ -312,13 +269,13 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 tc::commit(&s_full[t]);
             };
             auto outputs = [&](int t, int j) {  // O_t += P_t V_j
-                ok = ok && wait_phase(&p_full[t], static_cast<uint32_t>(j) & 1u, abort);
+                ok = ok && tc::wait_phase(&p_full[t], static_cast<uint32_t>(j) & 1u, abort);
                 if (!ok) return;
                 tc::fence_after();
 #pragma unroll
                 for (int sp = 0; sp < SPT; ++sp) {
                     const int e = v_seq(j) + sp, s = e % NST;
-                    ok = ok && wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
+                    ok = ok && tc::wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
                     if (!ok) return;
                     tc::fence_after();
                     const uint32_t vb = smem_u32(ring + s * C::kStage);
@@ -338,14 +295,14 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                         if (j >= nt[t]) continue;
                         outputs(t, j);
                         if (j + 1 < nt[t]) {
-                            ok = ok && wait_phase(pv_done(t, j), pv_parity(j), abort);
+                            ok = ok && tc::wait_phase(pv_done(t, j), pv_parity(j), abort);
                             if (ok) scores(t, j + 1);
                         }
                     }
                 } else {
                     for (int t = 0; t < NQ; ++t) {
                         if (j + 1 >= nt[t]) continue;
-                        ok = ok && wait_phase(&s_free[t], static_cast<uint32_t>(j) & 1u, abort);
+                        ok = ok && tc::wait_phase(&s_free[t], static_cast<uint32_t>(j) & 1u, abort);
                         if (!ok) break;
                         tc::fence_after();
                         scores(t, j + 1);
@@ -354,7 +311,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                         if (j < nt[t]) outputs(t, j);
                 }
             }
-            if (!ok) give_up(abort, a.err);
+            if (!ok) tc::give_up(abort, a.err);
             // every product has completed before tensor memory is freed
             tc::commit(drain);
             (void)mbar_wait_timed(drain, 0u);
@@ -395,7 +352,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         bool ok = true;
         for (int j = 0; j < nj; ++j) {
             const uint32_t par = static_cast<uint32_t>(j) & 1u;
-            ok = __all_sync(0xffffffffu, wait_phase(&s_full[t], par, abort));
+            ok = __all_sync(0xffffffffu, tc::wait_phase(&s_full[t], par, abort));
             if (!ok) break;
             tc::fence_after();
             float x[kKeys];
@@ -412,7 +369,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             // The product that last read this P buffer has been added (with one
             // buffer in S's columns, these scores came after it).
             if (!C::kAlias && j >= C::NP) {
-                ok = __all_sync(0xffffffffu, wait_phase(pv_done(t, j - C::NP), pv_parity(j - C::NP), abort));
+                ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - C::NP), pv_parity(j - C::NP), abort));
                 if (!ok) break;
                 tc::fence_after();
             }
@@ -428,11 +385,11 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
 #pragma unroll
             for (int c = 1; c < kKeys; ++c) top = fmaxf(top, x[c]);
             if (__any_sync(0xffffffffu, top > m + slack)) {
-                const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2((m - mn) * wk.scale2);
+                const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : tc::ex2((m - mn) * wk.scale2);
                 m = mn;
                 l *= f;
                 if (j > 0) {
-                    ok = __all_sync(0xffffffffu, wait_phase(pv_done(t, j - 1), pv_parity(j - 1), abort));
+                    ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - 1), pv_parity(j - 1), abort));
                     if (!ok) break;
                     tc::fence_after();
 #pragma unroll 1
@@ -454,7 +411,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < kKeys; c += 2) {
-                const float p0 = ex2(fmaf(x[c], wk.scale2, -m2)), p1 = ex2(fmaf(x[c + 1], wk.scale2, -m2));
+                const float p0 = tc::ex2(fmaf(x[c], wk.scale2, -m2)), p1 = tc::ex2(fmaf(x[c + 1], wk.scale2, -m2));
                 sum[(c >> 1) & 1] += p0;
                 sum[2 + ((c >> 1) & 1)] += p1;
                 p[c / 2] = pack16(p0, p1, T());
@@ -467,14 +424,14 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 const int q = j0 + (warp & 3) * 32 + lane;
                 // entries up to V of the tile before have landed: full's parity is unambiguous
                 if (C::NP == 2 && j > 0) {
-                    ok = __all_sync(0xffffffffu, wait_phase(pv_done(t, j - 1), pv_parity(j - 1), abort));
+                    ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - 1), pv_parity(j - 1), abort));
                     if (!ok) break;
                 }
                 const bool dead = q > t_max || (a.window > 0 && q < walk.w_min && q >= a.sinks);
 #pragma unroll
                 for (int sp = 0; sp < SPT; ++sp) {
                     const int e = v_seq(j) + sp, s = e % NST;
-                    ok = ok && __all_sync(0xffffffffu, wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort));
+                    ok = ok && __all_sync(0xffffffffu, tc::wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort));
                     if (!ok) break;
                     if (dead) {
                         uint4* row = reinterpret_cast<uint4*>(ring + s * C::kStage + (q - j0) * 128);
@@ -491,8 +448,8 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[t]);
         }
-        if (ok && nj > 0) ok = __all_sync(0xffffffffu, wait_phase(pv_done(t, nj - 1), pv_parity(nj - 1), abort));
-        if (!ok) give_up(abort, a.err);
+        if (ok && nj > 0) ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, nj - 1), pv_parity(nj - 1), abort));
+        if (!ok) tc::give_up(abort, a.err);
         tc::fence_after();
         constexpr int CS = D + 4;
         const int64_t item = bid;
@@ -582,9 +539,11 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
     }
 }
 
+}  // namespace
+
 // A pool as a 4-D tensor (column, slot, head, page); boxes of min(page, 128)
 // slots x 64 columns in the 128-byte swizzle.
-bool pool_map(const PagedKv& kv, void* pool, CUtensorMap* out) {
+bool paged_pool_map(const PagedKv& kv, void* pool, CUtensorMap* out) {
     const TmapEncodeFn encode = tmap_encoder();
     if (!encode) return false;
     const cuuint64_t page = cuuint64_t{1} << kv.page_log2;
@@ -602,6 +561,8 @@ bool pool_map(const PagedKv& kv, void* pool, CUtensorMap* out) {
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+namespace {
+
 template <typename T, int D>
 cudaError_t launch(const PagedKv& kv, const PagedAttn& a, PromptWork wk, int num_sms, cudaStream_t s) {
     using C = PCfg<D>;
@@ -616,7 +577,7 @@ cudaError_t launch(const PagedKv& kv, const PagedAttn& a, PromptWork wk, int num
         if (dev < 64) done[dev] = true;
     }
     CUtensorMap tk, tv;
-    if (!pool_map(kv, kv.k, &tk) || !pool_map(kv, kv.v, &tv)) return cudaErrorInvalidValue;
+    if (!paged_pool_map(kv, kv.k, &tk) || !paged_pool_map(kv, kv.v, &tv)) return cudaErrorInvalidValue;
     const int64_t rows = std::min<int64_t>(a.max_new, a.rows) * a.G;
     wk.tiles = static_cast<int>((rows + C::NQ * kRows - 1) / (C::NQ * kRows));
     const int64_t items = static_cast<int64_t>(wk.tiles) * kv.nseq * kv.nkv;

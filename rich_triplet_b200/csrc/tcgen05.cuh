@@ -3,6 +3,7 @@
 // operand in shared or tensor memory, tensor-memory loads and stores.
 #pragma once
 
+#include <cuda.h>  // CUtensorMap
 #include <stdint.h>
 
 #include "common.cuh"
@@ -60,6 +61,50 @@ __device__ __forceinline__ void alloc(uint32_t* slot, uint32_t cols) {  // one w
 }
 __device__ __forceinline__ void dealloc(uint32_t base, uint32_t cols) {  // one warp
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+}
+
+// Four-dimensional tensor copy into this CTA's shared memory, completing on `bar`.
+__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* tm, int x, int slot, int head, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Wait for phase `parity` of `bar`; gives up after a second or once *abort is set.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    const uint32_t addr = smem_u32(bar);
+    uint64_t t0 = 0;
+    for (uint32_t it = 1;; ++it) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((it & 1023u) == 0u) {
+            if (*abort) return false;
+            uint64_t t;
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+            if (it == 1024u) t0 = t;
+            else if (t - t0 > 1000000000ull) return false;
+        }
+    }
+}
+
+__device__ __forceinline__ void give_up(volatile int* abort, int* err) {
+    *abort = 1;
+    if (err) atomicExch(err, kErrMbarTimeout);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // 32 consecutive 32-bit columns of this thread's lane; the values are there after wait_ld.
