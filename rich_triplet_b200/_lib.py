@@ -6,6 +6,7 @@ loading fails loudly when it is missing -- there is no CPU fallback.
 
 import ctypes
 import os
+import struct
 import subprocess
 import threading
 
@@ -82,36 +83,12 @@ class RtQwen35Layer(ctypes.Structure):
                                                "norm_weight", "q", "k", "v", "o", "q_norm", "k_norm")]
 
 
-class RtPagedKv(ctypes.Structure):
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
-               [(n, ctypes.c_int64) for n in ("page_stride", "head_stride", "slot_stride", "num_pages")] + \
-               [(n, ctypes.c_int32) for n in ("fmt", "kv_heads", "head_dim", "page_size")] + \
-               [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32),
-                ("num_seqs", ctypes.c_int32), ("lens", ctypes.c_void_p)]
-
-
-class RtPagedRows(ctypes.Structure):
-    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
-               [(n, ctypes.c_int64) for n in ("row_stride", "head_stride", "rows")] + \
-               [("src_fmt", ctypes.c_int32), ("q_start", ctypes.c_void_p)]
-
-
-class RtPagedAttn(ctypes.Structure):
-    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p)] + \
-               [(n, ctypes.c_int64) for n in ("q_row_stride", "q_head_stride", "out_row_stride", "out_head_stride")] + \
-               [("lse", ctypes.c_void_p), ("lse_row_stride", ctypes.c_int64), ("rows", ctypes.c_int64)] + \
-               [(n, ctypes.c_int32) for n in ("num_heads", "window", "sinks", "max_new")] + \
-               [("scale", ctypes.c_float), ("mass_cap", ctypes.c_int32), ("q_start", ctypes.c_void_p),
-                ("mass", ctypes.c_void_p), ("mass_seq_stride", ctypes.c_int64), ("mass_head_stride", ctypes.c_int64),
-                ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_uint64)]
-
-
-class RtPagedEvict(ctypes.Structure):
-    _fields_ = [("mass", ctypes.c_void_p), ("mass_out", ctypes.c_void_p), ("mass_seq_stride", ctypes.c_int64),
-                ("mass_head_stride", ctypes.c_int64)] + \
-               [(n, ctypes.c_int32) for n in ("mass_cap", "budget", "sinks", "recent")] + \
-               [("dst_table", ctypes.c_void_p), ("dst_stride", ctypes.c_int64), ("kept", ctypes.c_void_p),
-                ("new_lens", ctypes.c_void_p)]
+# The rt_paged_* argument structs, packed with native alignment (a packed bytes
+# object is passed where the C ABI takes a pointer to the struct).
+RT_PAGED_KV = struct.Struct("@2P4q4iPq2iP")         # rt_paged_kv
+RT_PAGED_ROWS = struct.Struct("@2P3qiP")            # rt_paged_rows
+RT_PAGED_ATTN = struct.Struct("@2P4qP2q4ifi2P2qPQ")  # rt_paged_attn
+RT_PAGED_EVICT = struct.Struct("@2P2q4iPq2P")       # rt_paged_evict_args
 
 
 _vp = ctypes.c_void_p

@@ -593,4 +593,4 @@ def test_prompt_more_row_tiles_than_sms():
         check_prompt([2600, 900], [2000, 900], 16, 4, 256, 64, F16, window=1024, sinks=4, seed=5)
         check_prompt([2600, 900], [2000, 900], 16, 4, 128, 64, BF16, seed=6)
     from rich_triplet_b200 import paged
-    paged._context(torch.device("cuda", torch.cuda.current_device())).sync()  # raises if a wait gave up
+    paged.context(DEV).sync()  # raises if a wait gave up
