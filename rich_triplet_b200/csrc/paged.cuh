@@ -115,7 +115,7 @@ cudaError_t paged_decode_launch(const PagedKv& kv, const PagedAttn& a, void* wor
                                 cudaStream_t s);
 size_t paged_prompt_part_bytes(int num_sms);
 bool paged_pool_map(const PagedKv& kv, void* pool, CUtensorMap* out);
-cudaError_t paged_prompt_mass16_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s);
+cudaError_t paged_prompt_mass16_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s);
 cudaError_t paged_prompt16_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s);
 cudaError_t paged_prompt_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s);
 cudaError_t paged_evict_launch(const PagedKv& kv, const PagedEvict& e, cudaStream_t s);

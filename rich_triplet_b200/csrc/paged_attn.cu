@@ -123,7 +123,7 @@ cudaError_t mass(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
 cudaError_t paged_prompt_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s) {
     cudaError_t e = kv.type == kPagedF32 ? attend<float>(kv, a, s) : paged_prompt16_launch(kv, a, workspace, num_sms, s);
     if (e != cudaSuccess || !a.mass) return e;
-    return kv.type == kPagedF32 ? mass<float>(kv, a, s) : paged_prompt_mass16_launch(kv, a, s);
+    return kv.type == kPagedF32 ? mass<float>(kv, a, s) : paged_prompt_mass16_launch(kv, a, workspace, num_sms, s);
 }
 
 }  // namespace rt

@@ -15,6 +15,11 @@
 // tensor-memory buffers, and two warpgroups take alternate tiles.  Tiles of
 // early positions, which most rows see, start first.
 //
+// With a window, the tiles of the first tokens are seen by every row and the
+// others by a window's worth: their walks are split over several CTAs, and so
+// are all walks when there are few; the last of a walk's CTAs to finish adds
+// the parts in order.
+//
 // Waits are bounded as in paged_prompt.cu.
 #include <math.h>
 
@@ -32,6 +37,17 @@ constexpr int kTile = 128;     // positions, and rows, of a tile
 constexpr int kSumGroups = 2;  // warpgroups that add
 constexpr int kBufs = 4;       // score buffers in tensor memory
 constexpr int kThreads = (kSumGroups * 4 + 4 + 1) * 32;
+constexpr int kMaxParts = 16;  // CTAs that share a walk, at most
+
+// Grid: `first_parts` CTAs for each item (position tile, sequence and KV head)
+// below `first_items`, then `parts` for each other one.
+struct MassWork {
+    float* part;    // [item][kMaxParts][128]
+    uint32_t* cnt;  // [item], zero between calls
+    int64_t first_items;
+    int first_parts, parts;
+    float scale2;   // scale * log2(e)
+};
 
 template <int D>
 struct MCfg {
@@ -50,7 +66,7 @@ struct MCfg {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    paged_prompt_mass_kernel(const __grid_constant__ CUtensorMap tm_k, const PagedKv kv, const PagedAttn a, const float scale2) {
+    paged_prompt_mass_kernel(const __grid_constant__ CUtensorMap tm_k, const PagedKv kv, const PagedAttn a, const MassWork wk) {
     using C = MCfg<D>;
     constexpr int NST = C::NST;
     constexpr bool BF16 = !std::is_same<T, __half>::value;
@@ -59,8 +75,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- the positions of this CTA and the rows that see one of them ----
     const int G = a.G;
     const int64_t bhs = static_cast<int64_t>(kv.nseq) * kv.nkv;
-    const int j0 = static_cast<int>(blockIdx.x / bhs) * kTile;
-    const int b = static_cast<int>(blockIdx.x % bhs) / kv.nkv, h = static_cast<int>(blockIdx.x % bhs) % kv.nkv;
+    int64_t item = blockIdx.x;
+    int part, parts;
+    if (item < wk.first_items * wk.first_parts) {
+        parts = wk.first_parts;
+        part = static_cast<int>(item % parts);
+        item /= parts;
+    } else {
+        item -= wk.first_items * wk.first_parts;
+        parts = wk.parts;
+        part = static_cast<int>(item % parts);
+        item = item / parts + wk.first_items;
+    }
+    const int j0 = static_cast<int>(item / bhs) * kTile;
+    const int b = static_cast<int>(item % bhs) / kv.nkv, h = static_cast<int>(item % bhs) % kv.nkv;
     const int64_t q_first = a.q_start[b];
     const int all = a.q_start[b + 1] - static_cast<int>(q_first), len = kv.len(b);
     if (all <= 0 || q_first < 0) return;
@@ -72,8 +100,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (a.window > 0 && j0 >= a.sinks)
         i_hi = static_cast<int>(min(static_cast<int64_t>(i_hi), static_cast<int64_t>(j_end) - 1 + a.window - 1 - pos0));
     if (j_end <= j0 || i_hi < i_lo) return;
-    const int r_begin = i_lo * G, r_end = (i_hi + 1) * G;  // rows * G fits 32 bits (checked by the caller)
-    const int n = (r_end - r_begin + kTile - 1) / kTile;
+    // rows * G fits 32 bits (checked by the caller)
+    const int all_tiles = ((i_hi + 1 - i_lo) * G + kTile - 1) / kTile;
+    parts = min(parts, all_tiles);
+    if (part >= parts) return;
+    const int tile0 = static_cast<int>(static_cast<int64_t>(all_tiles) * part / parts);
+    const int n = static_cast<int>(static_cast<int64_t>(all_tiles) * (part + 1) / parts) - tile0;
+    const int r_begin = i_lo * G + tile0 * kTile, r_end = (i_hi + 1) * G;
 
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
     uint8_t* ring = sm + C::kOffRing;
@@ -85,6 +118,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* drain = k_full + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::kOffMisc);
     volatile int* abort = reinterpret_cast<volatile int*>(sm + C::kOffMisc + 4);
+    int* joined = reinterpret_cast<int*>(sm + C::kOffMisc + 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x & 127;
     if (threadIdx.x == 0) {
         for (int s = 0; s < NST; ++s) {
@@ -147,24 +181,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
     } else if (warp >= kSumGroups * 4) {
         // ---- query rows into the ring, one tile ahead of the one that is handed over ----
-        constexpr int CPR = D / 8;
+        constexpr int CPR = D / 8;          // 16-byte chunks of a row
+        constexpr int RPI = 32 / CPR;       // rows of a warp-wide copy
+        const int row0 = (warp & 3) * 32;   // this warp's rows of a tile
         bool ok = true;
         for (int i = 0; i <= n; ++i) {
             if (i < n) {
                 const int s = i % NST;
                 ok = ok && __all_sync(0xffffffffu, i < NST || tc::wait_phase(&empty[s], static_cast<uint32_t>(i / NST - 1) & 1u, abort));
                 if (!ok) break;
-                const uint32_t dst = smem_u32(ring + s * C::kOperand);
-                const int r0 = r_begin + i * kTile;
+                // rows past the end repeat the last one (their weight is 0)
+                const int rho = min(r_begin + i * kTile + row0 + lane, r_end - 1), tok = rho / G;
+                const int64_t off = (q_first + tok) * a.q_row + (h * G + rho - tok * G) * a.q_head;
+                const int ch = lane % CPR;
+                const T* src = static_cast<const T*>(a.q) + ch * 8;
+                const uint32_t dst = smem_u32(ring + s * C::kOperand) + (ch >> 3) * C::kChunk;
 #pragma unroll 8
-                for (int x = tid; x < kTile * CPR; x += 128) {
-                    const int row = x / CPR, ch = x % CPR;
-                    const int rho = min(r0 + row, r_end - 1), tok = rho / G;
-                    const T* src = static_cast<const T*>(a.q) + (q_first + tok) * a.q_row +
-                                   (h * G + rho - tok * G) * a.q_head + ch * 8;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                                     dst + (ch >> 3) * C::kChunk + row * 128 + (((ch & 7) ^ (row & 7)) << 4)),
-                                 "l"(src)
+                for (int x = 0; x < 32 / RPI; ++x) {
+                    const int r = x * RPI + lane / CPR, row = row0 + r;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4)),
+                                 "l"(src + __shfl_sync(0xffffffffu, off, r))
                                  : "memory");
                 }
             }
@@ -233,8 +269,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     const float4 z = *reinterpret_cast<const float4*>(&rb[c + e]);
-                    part[e & 2] += tc::ex2(fmaf(x[e], scale2, -z.x));
-                    part[(e & 2) + 1] += tc::ex2(fmaf(x[e + 1], scale2, -z.z));
+                    part[e & 2] += tc::ex2(fmaf(x[e], wk.scale2, -z.x));
+                    part[(e & 2) + 1] += tc::ex2(fmaf(x[e + 1], wk.scale2, -z.z));
                 }
             }
             total += (part[0] + part[1]) + (part[2] + part[3]);
@@ -246,9 +282,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (warp < 4) {
         const int j = j0 + threadIdx.x;
-        if (j < j_end && !*abort)
-            a.mass[b * a.mass_seq + h * a.mass_head + j] +=
-                total + reinterpret_cast<const float*>(sm + C::kOffTotal)[threadIdx.x];
+        float sum = total + reinterpret_cast<const float*>(sm + C::kOffTotal)[threadIdx.x];
+        bool write = j < j_end && !*abort;
+        if (parts > 1) {
+            float* pp = wk.part + item * kMaxParts * kTile + threadIdx.x;
+            __stcg(pp + part * kTile, sum);
+            __threadfence();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (threadIdx.x == 0) {
+                *joined = atomicAdd(&wk.cnt[item], 1u) == static_cast<uint32_t>(parts - 1);
+                if (*joined) wk.cnt[item] = 0u;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            write = write && *joined;
+            if (write) {
+                __threadfence();
+                sum = 0.f;
+                for (int q = 0; q < parts; ++q) sum += __ldcg(pp + q * kTile);
+            }
+        }
+        if (write) a.mass[b * a.mass_seq + h * a.mass_head + j] += sum;
     }
     if (warp == 0) {
         tc::fence_after();
@@ -257,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <typename T, int D>
-cudaError_t launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
+cudaError_t launch(const PagedKv& kv, const PagedAttn& a, MassWork wk, int num_sms, cudaStream_t s) {
     using C = MCfg<D>;
     auto kernel = paged_prompt_mass_kernel<T, D>;
     static bool done[64] = {};
@@ -272,24 +325,36 @@ cudaError_t launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
     CUtensorMap tk;
     if (!paged_pool_map(kv, kv.k, &tk)) return cudaErrorInvalidValue;
     const int64_t cap = std::min<int64_t>(static_cast<int64_t>(kv.width) << kv.page_log2, a.mass_cap);
-    const int64_t grid = (cap + kTile - 1) / kTile * kv.nseq * kv.nkv;
-    if (grid == 0) return cudaSuccess;
+    const int64_t bhs = static_cast<int64_t>(kv.nseq) * kv.nkv, tiles = (cap + kTile - 1) / kTile, items = tiles * bhs;
+    if (items == 0) return cudaSuccess;
+    auto share = [&](int64_t walks) {  // CTAs of a walk when there are so many
+        return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxParts, num_sms / walks)));
+    };
+    wk.parts = share(items);
+    wk.first_items = a.window > 0 ? std::min<int64_t>(tiles, (static_cast<int64_t>(a.sinks) + kTile - 1) / kTile) * bhs : 0;
+    wk.first_parts = wk.first_items > 0 ? std::max(wk.parts, share(wk.first_items)) : 1;
+    const int64_t grid = wk.first_items * wk.first_parts + (items - wk.first_items) * wk.parts;
     if (grid > INT32_MAX) return cudaErrorInvalidValue;
-    kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmem, s>>>(tk, kv, a, a.scale * 1.44269504088896341f);
+    kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmem, s>>>(tk, kv, a, wk);
     return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t by_dim(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
-    if (kv.D == 64) return launch<T, 64>(kv, a, s);
-    if (kv.D == 128) return launch<T, 128>(kv, a, s);
-    return launch<T, 256>(kv, a, s);
+cudaError_t by_dim(const PagedKv& kv, const PagedAttn& a, const MassWork& wk, int num_sms, cudaStream_t s) {
+    if (kv.D == 64) return launch<T, 64>(kv, a, wk, num_sms, s);
+    if (kv.D == 128) return launch<T, 128>(kv, a, wk, num_sms, s);
+    return launch<T, 256>(kv, a, wk, num_sms, s);
 }
 
 }  // namespace
 
-cudaError_t paged_prompt_mass16_launch(const PagedKv& kv, const PagedAttn& a, cudaStream_t s) {
-    return kv.type == kPagedF16 ? by_dim<__half>(kv, a, s) : by_dim<__nv_bfloat16>(kv, a, s);
+cudaError_t paged_prompt_mass16_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s) {
+    MassWork wk = {};
+    wk.cnt = static_cast<uint32_t*>(workspace);
+    wk.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + paged_counter_bytes(num_sms));
+    wk.scale2 = a.scale * 1.44269504088896341f;
+    static_assert(kMaxParts * kTile <= 2 * 128 * (128 + 4), "fits paged_prompt_part_bytes");
+    return kv.type == kPagedF16 ? by_dim<__half>(kv, a, wk, num_sms, s) : by_dim<__nv_bfloat16>(kv, a, wk, num_sms, s);
 }
 
 }  // namespace rt

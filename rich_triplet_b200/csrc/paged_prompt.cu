@@ -53,6 +53,8 @@ namespace {
 constexpr int kKeys = 128;   // positions of a key tile
 constexpr int kRows = 128;   // rows of a query tile
 constexpr float kMaxSlack = 8.f;
+constexpr int kSoftRegs = 208, kOtherRegs = 88;
+constexpr int kMaxSplit = 16;  // CTAs that share a walk, at most
 
 template <int D>
 struct PCfg {
@@ -67,11 +69,14 @@ struct PCfg {
     static constexpr int kQTile = (D / 64) * kChunk;
     static constexpr int kOffRing = NQ * kQTile;
     static constexpr int kOffBar = kOffRing + NST * kStage;
-    static constexpr int kBars = 2 * NST + (3 + NP) * NQ + 2;
+    static constexpr int kBars = 2 * NST + (2 + 3 * NP) * NQ + 2;
     static constexpr int kOffMisc = kOffBar + kBars * 8;
     static constexpr int kSmem = kOffMisc + 16 + 1024;  // + alignment of the tiles
     static constexpr int kSoftWarps = 4 * NQ;
-    static constexpr int kThreads = (kSoftWarps + 2) * 32;
+    // With two query tiles the warps are 3 warpgroups of 168 registers a
+    // thread, of which the third (producer, MMA, two idle warps) gives up 80 so
+    // that the softmax threads have 208 (2 x 208 + 88 = 3 x 168).
+    static constexpr int kThreads = NQ == 2 ? 384 : (kSoftWarps + 2) * 32;
     static constexpr uint32_t kS = D == 64 ? 128 : 256;                // S of query tile 0; the next 128 columns on
     static constexpr uint32_t kP = D == 128 ? kS : 384;                // P buffers 64 columns apart
     __host__ __device__ static constexpr uint32_t o_col(int t) { return static_cast<uint32_t>(t * D); }
@@ -160,10 +165,10 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
     uint64_t* empty = full + NST;
     uint64_t* s_full = empty + NST;   // [NQ] scores are in tensor memory
     uint64_t* s_free = s_full + NQ;   // [NQ] they have been read
-    uint64_t* p_full = s_free + NQ;   // [NQ] the weights are there, the output is rescaled
-    // [NQ][NP] their product with V has been added: one barrier per P buffer, so
-    // that a waiter is never two phases behind (a parity could not tell)
-    uint64_t* pv_bars = p_full + NQ;
+    // One barrier per P buffer, so that no waiter is ever two phases behind (a parity could not tell):
+    uint64_t* half_bars = s_free + NQ;              // [NQ][NP] the weights of the first 64 positions are there, the output is rescaled
+    uint64_t* full_bars = half_bars + NQ * C::NP;   // [NQ][NP] the other 64 too
+    uint64_t* pv_bars = full_bars + NQ * C::NP;     // [NQ][NP] their product with V has been added
     uint64_t* q_full = pv_bars + NQ * C::NP;
     uint64_t* drain = q_full + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::kOffMisc);
@@ -178,8 +183,11 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         for (int t = 0; t < NQ; ++t) {
             mbar_init(&s_full[t], 1);
             mbar_init(&s_free[t], 4);
-            mbar_init(&p_full[t], 4);
-            for (int i = 0; i < C::NP; ++i) mbar_init(&pv_bars[t * C::NP + i], 1);
+            for (int i = t * C::NP; i < (t + 1) * C::NP; ++i) {
+                mbar_init(&half_bars[i], 4);
+                mbar_init(&full_bars[i], 4);
+                mbar_init(&pv_bars[i], 1);
+            }
         }
         mbar_init(q_full, C::kSoftWarps);
         mbar_init(drain, 1);
@@ -192,14 +200,18 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
     tc::fence_after();
     const uint32_t tmem = *tmem_slot;
 
+    auto p_half = [&](int t, int j) { return &half_bars[t * C::NP + j % C::NP]; };
+    auto p_full = [&](int t, int j) { return &full_bars[t * C::NP + j % C::NP]; };
     auto pv_done = [&](int t, int j) { return &pv_bars[t * C::NP + j % C::NP]; };
-    auto pv_parity = [](int j) { return static_cast<uint32_t>(j / C::NP) & 1u; };
+    auto p_parity = [](int j) { return static_cast<uint32_t>(j / C::NP) & 1u; };
 
     // Ring order of the tiles: K0, K1, V0, K2, V1, ... (scores run a tile
     // ahead), or K0, V0, K1, V1, ... where P shares S's columns.
     auto k_seq = [&](int j) { return SPT * (C::kAlias ? 2 * j : (j == 0 ? 0 : 2 * j - 1)); };
     auto v_seq = [&](int j) { return SPT * (C::kAlias ? 2 * j + 1 : (j + 1 < n ? 2 * j + 2 : 2 * j + 1)); };
 
+    if (warp >= C::kSoftWarps) {
+    if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == C::kSoftWarps) {
         // ---- producer ----
         const int rows = min(1 << kv.page_log2, kKeys), boxes = kKeys / rows;
@@ -268,22 +280,28 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 }
                 tc::commit(&s_full[t]);
             };
-            auto outputs = [&](int t, int j) {  // O_t += P_t V_j
-                ok = ok && tc::wait_phase(&p_full[t], static_cast<uint32_t>(j) & 1u, abort);
-                if (!ok) return;
-                tc::fence_after();
+            auto outputs = [&](int t, int j) {  // O_t += P_t V_j, as the halves of P_t come
+                ok = ok && tc::wait_phase(p_half(t, j), p_parity(j), abort);
 #pragma unroll
-                for (int sp = 0; sp < SPT; ++sp) {
-                    const int e = v_seq(j) + sp, s = e % NST;
-                    ok = ok && tc::wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
+                for (int half = 0; half < 2; ++half) {
+                    if (half) ok = ok && tc::wait_phase(p_full(t, j), p_parity(j), abort);
                     if (!ok) return;
                     tc::fence_after();
-                    const uint32_t vb = smem_u32(ring + s * C::kStage);
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        tc::mma_ts(tmem + C::o_col(t) + sp * C::SD, tmem + C::p_col(t, j) + 8 * k,
-                                   tc::desc_sw128(vb + k * 2048, C::kChunk), kIdO, j > 0 || k > 0);
-                    if (t == last_t(j)) tc::commit(&empty[s]);
+                    for (int sp = 0; sp < SPT; ++sp) {
+                        const int e = v_seq(j) + sp, s = e % NST;
+                        if (!half) {
+                            ok = ok && tc::wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
+                            if (!ok) return;
+                            tc::fence_after();
+                        }
+                        const uint32_t vb = smem_u32(ring + s * C::kStage);
+#pragma unroll
+                        for (int k = 4 * half; k < 4 * half + 4; ++k)
+                            tc::mma_ts(tmem + C::o_col(t) + sp * C::SD, tmem + C::p_col(t, j) + 8 * k,
+                                       tc::desc_sw128(vb + k * 2048, C::kChunk), kIdO, j > 0 || k > 0);
+                        if (half && t == last_t(j)) tc::commit(&empty[s]);
+                    }
                 }
                 tc::commit(pv_done(t, j));
             };
@@ -295,7 +313,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                         if (j >= nt[t]) continue;
                         outputs(t, j);
                         if (j + 1 < nt[t]) {
-                            ok = ok && tc::wait_phase(pv_done(t, j), pv_parity(j), abort);
+                            ok = ok && tc::wait_phase(pv_done(t, j), p_parity(j), abort);
                             if (ok) scores(t, j + 1);
                         }
                     }
@@ -317,8 +335,10 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             (void)mbar_wait_timed(drain, 0u);
         }
         __syncwarp();
+    }
     } else {
         // ---- one warpgroup per query tile, one thread per row ----
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int t = warp >> 2, r = t * kRows + (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // tensor-memory lane 32 (warp % 4), bits 16 on
         const int nj = tiles_of(t);
@@ -369,7 +389,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             // The product that last read this P buffer has been added (with one
             // buffer in S's columns, these scores came after it).
             if (!C::kAlias && j >= C::NP) {
-                ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - C::NP), pv_parity(j - C::NP), abort));
+                ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - C::NP), p_parity(j - C::NP), abort));
                 if (!ok) break;
                 tc::fence_after();
             }
@@ -381,15 +401,21 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 for (int c = 0; c < kKeys; ++c)
                     if (c > hi || (c <= lo && c >= first)) x[c] = -INFINITY;
             }
-            float top = x[0];
+            float top[4];
 #pragma unroll
-            for (int c = 1; c < kKeys; ++c) top = fmaxf(top, x[c]);
-            if (__any_sync(0xffffffffu, top > m + slack)) {
-                const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : tc::ex2((m - mn) * wk.scale2);
+            for (int q = 0; q < 4; ++q) {
+                top[q] = tc::max3(x[32 * q], x[32 * q + 1], x[32 * q + 2]);
+#pragma unroll
+                for (int c = 3; c < 31; c += 2) top[q] = tc::max3(top[q], x[32 * q + c], x[32 * q + c + 1]);
+                top[q] = fmaxf(top[q], x[32 * q + 31]);
+            }
+            top[0] = fmaxf(tc::max3(top[0], top[1], top[2]), top[3]);
+            if (__any_sync(0xffffffffu, top[0] > m + slack)) {
+                const float mn = fmaxf(m, top[0]), f = m == -INFINITY ? 0.f : tc::ex2((m - mn) * wk.scale2);
                 m = mn;
                 l *= f;
                 if (j > 0) {
-                    ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - 1), pv_parity(j - 1), abort));
+                    ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - 1), p_parity(j - 1), abort));
                     if (!ok) break;
                     tc::fence_after();
 #pragma unroll 1
@@ -407,24 +433,12 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 }
             }
             const float m2 = m == -INFINITY ? 0.f : m * wk.scale2;
-            uint32_t p[kKeys / 2];
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < kKeys; c += 2) {
-                const float p0 = tc::ex2(fmaf(x[c], wk.scale2, -m2)), p1 = tc::ex2(fmaf(x[c + 1], wk.scale2, -m2));
-                sum[(c >> 1) & 1] += p0;
-                sum[2 + ((c >> 1) & 1)] += p1;
-                p[c / 2] = pack16(p0, p1, T());
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tc::st32(tmem + lanes + C::p_col(t, j), p);
-            tc::st32(tmem + lanes + C::p_col(t, j) + 32, p + 32);
             // rows of V that no row of this CTA sees: zero (once, by the first query tile that uses them)
             if ((t == 0 || j >= tiles_of(0)) && (j0 + kKeys - 1 > t_max || (a.window > 0 && j0 < walk.w_min))) {
                 const int q = j0 + (warp & 3) * 32 + lane;
                 // entries up to V of the tile before have landed: full's parity is unambiguous
                 if (C::NP == 2 && j > 0) {
-                    ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - 1), pv_parity(j - 1), abort));
+                    ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - 1), p_parity(j - 1), abort));
                     if (!ok) break;
                 }
                 const bool dead = q > t_max || (a.window > 0 && q < walk.w_min && q >= a.sinks);
@@ -443,12 +457,35 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 if (!ok) break;
                 fence_proxy_async_smem();
             }
+            const float2 sc = make_float2(wk.scale2, wk.scale2), nm = make_float2(-m2, -m2);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            uint32_t p[kKeys / 4];
+            auto weights = [&](int q) {  // columns 32 q .. 32 q + 31
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    float2 w = ffma2(make_float2(x[32 * q + c], x[32 * q + c + 1]), sc, nm);
+                    w = make_float2(tc::ex2(w.x), tc::ex2(w.y));
+                    sum[(c >> 1) & 1] = tc::add2(sum[(c >> 1) & 1], w);
+                    p[16 * (q & 1) + c / 2] = pack16(w.x, w.y, T());
+                }
+            };
+            weights(0);
+            weights(1);
+            tc::st32(tmem + lanes + C::p_col(t, j), p);
+            weights(2);
             tc::wait_st();
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
+            if (lane == 0) mbar_arrive(p_half(t, j));
+            weights(3);
+            tc::st32(tmem + lanes + C::p_col(t, j) + 32, p);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(t, j));
         }
-        if (ok && nj > 0) ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, nj - 1), pv_parity(nj - 1), abort));
+        if (ok && nj > 0) ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, nj - 1), p_parity(nj - 1), abort));
         if (!ok) tc::give_up(abort, a.err);
         tc::fence_after();
         constexpr int CS = D + 4;
@@ -501,32 +538,51 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             if (*joined) {
                 __threadfence();
                 const float* recs = wk.part + item * wk.nsplit * NQ * kRows * CS;
+                constexpr int64_t kNext = static_cast<int64_t>(NQ) * kRows * CS;
+                // [row][split] weights, 1 / sum with the last one (in the ring, which is free)
+                float* wgt = reinterpret_cast<float*>(ring);
+                for (int row = threadIdx.x; row < nrows; row += kSoft) {
+                    const float* p = recs + static_cast<int64_t>(row) * CS + D;
+                    float M = -INFINITY, L = 0.f;
+                    float2 ml[kMaxSplit];
+#pragma unroll
+                    for (int s = 0; s < kMaxSplit; ++s)
+                        if (s < ns) {
+                            ml[s] = __ldcg(reinterpret_cast<const float2*>(p + s * kNext));
+                            M = fmaxf(M, ml[s].x);
+                        }
+#pragma unroll
+                    for (int s = 0; s < kMaxSplit; ++s)
+                        if (s < ns) {
+                            const float f = ml[s].x == -INFINITY ? 0.f : exp2f(ml[s].x - M);
+                            L += ml[s].y * f;
+                            wgt[row * (kMaxSplit + 1) + s] = f;
+                        }
+                    wgt[row * (kMaxSplit + 1) + kMaxSplit] = M == -INFINITY ? 0.f : 1.f / L;
+                    const int64_t rr = row0 + row, tk = rr / G;
+                    if (a.lse)
+                        a.lse[(q_first + tk) * a.lse_row + h * G + static_cast<int>(rr - tk * G)] =
+                            M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
                 for (int i = threadIdx.x; i < nrows * (D / 4); i += kSoft) {
                     const int row = i / (D / 4), d = (i % (D / 4)) * 4;
-                    const float* p = recs + static_cast<int64_t>(row) * CS;
-                    float M = -INFINITY, L = 0.f;
-                    for (int s = 0; s < ns; ++s) M = fmaxf(M, __ldcg(p + static_cast<int64_t>(s) * NQ * kRows * CS + D));
+                    const float* p = recs + static_cast<int64_t>(row) * CS + d;
+                    const float* f = wgt + row * (kMaxSplit + 1);
                     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
                     for (int s = 0; s < ns; ++s) {
-                        const float* ps = p + static_cast<int64_t>(s) * NQ * kRows * CS;
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(ps + D));
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(ps + d));
-                        const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-                        L += ml.y * f;
-                        A.x += v.x * f;
-                        A.y += v.y * f;
-                        A.z += v.z * f;
-                        A.w += v.w * f;
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(p + s * kNext));
+                        A.x += v.x * f[s];
+                        A.y += v.y * f[s];
+                        A.z += v.z * f[s];
+                        A.w += v.w * f[s];
                     }
                     const int64_t rr = row0 + row, tk = rr / G;
-                    const int hd = h * G + static_cast<int>(rr - tk * G);
-                    const float iv = M == -INFINITY ? 0.f : 1.f / L;
-                    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (q_first + tk) * a.out_row + hd * a.out_head + d) =
+                    const float iv = f[kMaxSplit];
+                    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (q_first + tk) * a.out_row +
+                                              (h * G + static_cast<int>(rr - tk * G)) * a.out_head + d) =
                         make_uint2(pack16(A.x * iv, A.y * iv, T()), pack16(A.z * iv, A.w * iv, T()));
-                    if (d == 0 && a.lse)
-                        a.lse[(q_first + tk) * a.lse_row + hd] =
-                            M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
                 }
             }
         }
@@ -583,7 +639,7 @@ cudaError_t launch(const PagedKv& kv, const PagedAttn& a, PromptWork wk, int num
     const int64_t items = static_cast<int64_t>(wk.tiles) * kv.nseq * kv.nkv;
     const int64_t key_tiles = ((static_cast<int64_t>(kv.width) << kv.page_log2) + kKeys - 1) / kKeys;
     // few rows: each walk over as many CTAs as fill the SMs, two key tiles each at least
-    wk.nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms / items, (key_tiles + 1) / 2)));
+    wk.nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({num_sms / items, (key_tiles + 1) / 2, kMaxSplit})));
     if (items * wk.nsplit > INT32_MAX) return cudaErrorInvalidValue;
     kernel<<<static_cast<unsigned>(items * wk.nsplit), C::kThreads, C::kSmem, s>>>(tk, tv, kv, a, wk);
     return cudaGetLastError();
