@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::kOffMisc);
     volatile int* abort = reinterpret_cast<volatile int*>(sm + C::kOffMisc + 4);
     int* joined = reinterpret_cast<int*>(sm + C::kOffMisc + 8);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x & 127;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tid = threadIdx.x & 127;
     if (threadIdx.x == 0) {
         for (int s = 0; s < NST; ++s) {
             mbar_init(&full[s], 4);
@@ -155,29 +155,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                        k_full);
         }
         __syncwarp();
-        if (lane == 0) {
-            constexpr uint32_t kId = tc::idesc_f16(BF16, kTile, false);
-            bool ok = tc::wait_phase(k_full, 0u, abort);
-            for (int i = 0; i < n && ok; ++i) {
-                const int s = i % NST, buf = i % kBufs;
-                ok = tc::wait_phase(&full[s], static_cast<uint32_t>(i / NST) & 1u, abort) &&
-                     (i < kBufs || tc::wait_phase(&s_free[buf], static_cast<uint32_t>(i / kBufs - 1) & 1u, abort));
-                if (!ok) break;
-                tc::fence_after();
-                const uint32_t kb = smem_u32(sm), qb = smem_u32(ring + s * C::kOperand);
+        constexpr uint32_t kId = tc::idesc_f16(BF16, kTile, false);
+        bool ok = tc::warp_wait(k_full, 0u, abort);
+        for (int i = 0; i < n && ok; ++i) {
+            const int s = i % NST, buf = i % kBufs;
+            ok = tc::warp_wait(&full[s], static_cast<uint32_t>(i / NST) & 1u, abort) &&
+                 (i < kBufs || tc::warp_wait(&s_free[buf], static_cast<uint32_t>(i / kBufs - 1) & 1u, abort));
+            if (!ok) break;
+            tc::fence_after();
+            const uint32_t kb = tc::uniform(tc::desc_lo(smem_u32(sm), 16)), st = tc::uniform(tmem + buf * kTile);
+            const uint32_t qb = tc::uniform(tc::desc_lo(smem_u32(ring + s * C::kOperand), 16));
+            if (tc::elect()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint32_t at = (k >> 2) * C::kChunk + (k & 3) * 32;
-                    tc::mma_ss(tmem + buf * kTile, tc::desc_sw128(kb + at, 16), tc::desc_sw128(qb + at, 16), kId, k > 0);
+                    tc::mma_ss(st, tc::desc_sw128(kb, at), tc::desc_sw128(qb, at), kId, k > 0);
                 }
                 tc::commit(&empty[s]);
                 tc::commit(&s_full[buf]);
             }
-            if (!ok) tc::give_up(abort, a.err);
-            tc::commit(drain);
-            (void)mbar_wait_timed(drain, 0u);
-            (void)mbar_wait_timed(k_full, 0u);
+            __syncwarp();
         }
+        if (!ok) tc::give_up(abort, a.err);
+        if (tc::elect()) tc::commit(drain);
+        __syncwarp();
+        (void)mbar_wait_timed(drain, 0u);
+        (void)mbar_wait_timed(k_full, 0u);
         __syncwarp();
     } else if (warp >= kSumGroups * 4) {
         // ---- query rows into the ring, one tile ahead of the one that is handed over ----
@@ -188,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i <= n; ++i) {
             if (i < n) {
                 const int s = i % NST;
-                ok = ok && __all_sync(0xffffffffu, i < NST || tc::wait_phase(&empty[s], static_cast<uint32_t>(i / NST - 1) & 1u, abort));
+                ok = ok && (i < NST || tc::warp_wait(&empty[s], static_cast<uint32_t>(i / NST - 1) & 1u, abort));
                 if (!ok) break;
                 // rows past the end repeat the last one (their weight is 0)
                 const int rho = min(r_begin + i * kTile + row0 + lane, r_end - 1), tok = rho / G;
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             load_rows(i + kSumGroups);
             const int buf = i % kBufs;
-            ok = __all_sync(0xffffffffu, tc::wait_phase(&s_full[buf], static_cast<uint32_t>(i / kBufs) & 1u, abort));
+            ok = tc::warp_wait(&s_full[buf], static_cast<uint32_t>(i / kBufs) & 1u, abort);
             if (!ok) break;
             tc::fence_after();
             const int r0 = r_begin + i * kTile, r1 = min(r0 + kTile, r_end) - 1;

@@ -52,7 +52,7 @@ namespace {
 
 constexpr int kKeys = 128;   // positions of a key tile
 constexpr int kRows = 128;   // rows of a query tile
-constexpr float kMaxSlack = 8.f;
+constexpr float kMaxSlack = 8.f, kMaxWeight = 256.f;  // how far weights may exceed 1 (powers of two; their sum)
 constexpr int kSoftRegs = 208, kOtherRegs = 88;
 constexpr int kMaxSplit = 16;  // CTAs that share a walk, at most
 
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::kOffMisc);
     volatile int* abort = reinterpret_cast<volatile int*>(sm + C::kOffMisc + 4);
     int* joined = reinterpret_cast<int*>(sm + C::kOffMisc + 8);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < NST; ++s) {
             mbar_init(&full[s], 1);
@@ -254,56 +254,64 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             for (int e = max(0, done - NST); e < done; ++e)
                 (void)mbar_wait_timed(&full[e % NST], static_cast<uint32_t>(e / NST) & 1u);
     } else if (warp == C::kSoftWarps + 1) {
-        if (lane == 0) {
-            // ---- MMA issuer ----
+        {
+            // ---- MMA issuer: the warp walks, one elected lane issues ----
             constexpr uint32_t kIdS = tc::idesc_f16(BF16, kKeys, false), kIdO = tc::idesc_f16(BF16, C::SD, true);
             int nt[NQ];
 #pragma unroll
             for (int t = 0; t < NQ; ++t) nt[t] = tiles_of(t);
             auto last_t = [&](int j) { return NQ == 2 && j < nt[NQ - 1] ? 1 : 0; };
-            bool ok = tc::wait_phase(q_full, 0u, abort);
+            bool ok = tc::warp_wait(q_full, 0u, abort);
             auto scores = [&](int t, int j) {  // S_t = Q_t K_j^T
 #pragma unroll
                 for (int sp = 0; sp < SPT; ++sp) {
                     const int e = k_seq(j) + sp, s = e % NST;
-                    ok = ok && tc::wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
+                    ok = ok && tc::warp_wait(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
                     if (!ok) return;
                     tc::fence_after();
-                    const uint32_t kb = smem_u32(ring + s * C::kStage), qb = smem_u32(sm + t * C::kQTile) + sp * C::kStage;
+                    const uint32_t kb = tc::uniform(tc::desc_lo(smem_u32(ring + s * C::kStage), 16));
+                    const uint32_t qb = tc::uniform(tc::desc_lo(smem_u32(sm + t * C::kQTile + sp * C::kStage), 16));
+                    const uint32_t st = tc::uniform(tmem + C::s_col(t));
+                    if (tc::elect()) {
 #pragma unroll
-                    for (int k = 0; k < C::SD / 16; ++k) {
-                        const uint32_t at = (k >> 2) * C::kChunk + (k & 3) * 32;
-                        tc::mma_ss(tmem + C::s_col(t), tc::desc_sw128(qb + at, 16), tc::desc_sw128(kb + at, 16), kIdS,
-                                   sp > 0 || k > 0);
+                        for (int k = 0; k < C::SD / 16; ++k) {
+                            const uint32_t at = (k >> 2) * C::kChunk + (k & 3) * 32;
+                            tc::mma_ss(st, tc::desc_sw128(qb, at), tc::desc_sw128(kb, at), kIdS, sp > 0 || k > 0);
+                        }
+                        if (t == last_t(j)) tc::commit(&empty[s]);
+                        if (sp == SPT - 1) tc::commit(&s_full[t]);
                     }
-                    if (t == last_t(j)) tc::commit(&empty[s]);
+                    __syncwarp();
                 }
-                tc::commit(&s_full[t]);
             };
             auto outputs = [&](int t, int j) {  // O_t += P_t V_j, as the halves of P_t come
-                ok = ok && tc::wait_phase(p_half(t, j), p_parity(j), abort);
+                ok = ok && tc::warp_wait(p_half(t, j), p_parity(j), abort);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    if (half) ok = ok && tc::wait_phase(p_full(t, j), p_parity(j), abort);
+                    if (half) ok = ok && tc::warp_wait(p_full(t, j), p_parity(j), abort);
                     if (!ok) return;
                     tc::fence_after();
 #pragma unroll
                     for (int sp = 0; sp < SPT; ++sp) {
                         const int e = v_seq(j) + sp, s = e % NST;
                         if (!half) {
-                            ok = ok && tc::wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
+                            ok = ok && tc::warp_wait(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
                             if (!ok) return;
                             tc::fence_after();
                         }
-                        const uint32_t vb = smem_u32(ring + s * C::kStage);
+                        const uint32_t vb = tc::uniform(tc::desc_lo(smem_u32(ring + s * C::kStage), C::kChunk));
+                        const uint32_t ot = tc::uniform(tmem + C::o_col(t) + sp * C::SD), pt = tc::uniform(tmem + C::p_col(t, j));
+                        const uint32_t more = tc::uniform(j > 0);
+                        if (tc::elect()) {
 #pragma unroll
-                        for (int k = 4 * half; k < 4 * half + 4; ++k)
-                            tc::mma_ts(tmem + C::o_col(t) + sp * C::SD, tmem + C::p_col(t, j) + 8 * k,
-                                       tc::desc_sw128(vb + k * 2048, C::kChunk), kIdO, j > 0 || k > 0);
-                        if (half && t == last_t(j)) tc::commit(&empty[s]);
+                            for (int k = 4 * half; k < 4 * half + 4; ++k)
+                                tc::mma_ts(ot, pt + 8 * k, tc::desc_sw128(vb, k * 2048), kIdO, k > 0 ? 1u : more);
+                            if (half && t == last_t(j)) tc::commit(&empty[s]);
+                            if (half && sp == SPT - 1) tc::commit(pv_done(t, j));
+                        }
+                        __syncwarp();
                     }
                 }
-                tc::commit(pv_done(t, j));
             };
             for (int t = 0; t < NQ; ++t)
                 if (nt[t] > 0) scores(t, 0);
@@ -313,14 +321,14 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                         if (j >= nt[t]) continue;
                         outputs(t, j);
                         if (j + 1 < nt[t]) {
-                            ok = ok && tc::wait_phase(pv_done(t, j), p_parity(j), abort);
+                            ok = ok && tc::warp_wait(pv_done(t, j), p_parity(j), abort);
                             if (ok) scores(t, j + 1);
                         }
                     }
                 } else {
                     for (int t = 0; t < NQ; ++t) {
                         if (j + 1 >= nt[t]) continue;
-                        ok = ok && tc::wait_phase(&s_free[t], static_cast<uint32_t>(j) & 1u, abort);
+                        ok = ok && tc::warp_wait(&s_free[t], static_cast<uint32_t>(j) & 1u, abort);
                         if (!ok) break;
                         tc::fence_after();
                         scores(t, j + 1);
@@ -331,7 +339,8 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             }
             if (!ok) tc::give_up(abort, a.err);
             // every product has completed before tensor memory is freed
-            tc::commit(drain);
+            if (tc::elect()) tc::commit(drain);
+            __syncwarp();
             (void)mbar_wait_timed(drain, 0u);
         }
         __syncwarp();
@@ -341,7 +350,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
         const int t = warp >> 2, r = t * kRows + (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // tensor-memory lane 32 (warp % 4), bits 16 on
-        const int nj = tiles_of(t);
+        const int nj = tiles_of(t), n0 = tiles_of(0);
         {
             // Q tile t into shared memory, rows past the end zero
             constexpr int CPR = D / 8;  // 16-byte chunks of a row
@@ -367,12 +376,11 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         const int pos = live ? pos0 + tok : -1;
         const int tile_lo = pos0 + static_cast<int>((row0 + t * kRows) / G);
         const int tile_hi = pos0 + static_cast<int>((row0 + min(nrows, (t + 1) * kRows) - 1) / G);
-        const float slack = kMaxSlack / wk.scale2;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; j < nj; ++j) {
             const uint32_t par = static_cast<uint32_t>(j) & 1u;
-            ok = __all_sync(0xffffffffu, tc::wait_phase(&s_full[t], par, abort));
+            ok = tc::warp_wait(&s_full[t], par, abort);
             if (!ok) break;
             tc::fence_after();
             float x[kKeys];
@@ -389,7 +397,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             // The product that last read this P buffer has been added (with one
             // buffer in S's columns, these scores came after it).
             if (!C::kAlias && j >= C::NP) {
-                ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - C::NP), p_parity(j - C::NP), abort));
+                ok = tc::warp_wait(pv_done(t, j - C::NP), p_parity(j - C::NP), abort);
                 if (!ok) break;
                 tc::fence_after();
             }
@@ -401,51 +409,19 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 for (int c = 0; c < kKeys; ++c)
                     if (c > hi || (c <= lo && c >= first)) x[c] = -INFINITY;
             }
-            float top[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                top[q] = tc::max3(x[32 * q], x[32 * q + 1], x[32 * q + 2]);
-#pragma unroll
-                for (int c = 3; c < 31; c += 2) top[q] = tc::max3(top[q], x[32 * q + c], x[32 * q + c + 1]);
-                top[q] = fmaxf(top[q], x[32 * q + 31]);
-            }
-            top[0] = fmaxf(tc::max3(top[0], top[1], top[2]), top[3]);
-            if (__any_sync(0xffffffffu, top[0] > m + slack)) {
-                const float mn = fmaxf(m, top[0]), f = m == -INFINITY ? 0.f : tc::ex2((m - mn) * wk.scale2);
-                m = mn;
-                l *= f;
-                if (j > 0) {
-                    ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - 1), p_parity(j - 1), abort));
-                    if (!ok) break;
-                    tc::fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        float o[32];
-                        uint32_t u[32];
-                        tc::ld32(tmem + lanes + C::o_col(t) + c, o);
-                        tc::wait_ld();
-                        tc::tie32(o);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * f);
-                        tc::st32(tmem + lanes + C::o_col(t) + c, u);
-                    }
-                    tc::wait_st();
-                }
-            }
-            const float m2 = m == -INFINITY ? 0.f : m * wk.scale2;
             // rows of V that no row of this CTA sees: zero (once, by the first query tile that uses them)
-            if ((t == 0 || j >= tiles_of(0)) && (j0 + kKeys - 1 > t_max || (a.window > 0 && j0 < walk.w_min))) {
+            if ((t == 0 || j >= n0) && (j0 + kKeys - 1 > t_max || (a.window > 0 && j0 < walk.w_min))) {
                 const int q = j0 + (warp & 3) * 32 + lane;
                 // entries up to V of the tile before have landed: full's parity is unambiguous
                 if (C::NP == 2 && j > 0) {
-                    ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, j - 1), p_parity(j - 1), abort));
+                    ok = tc::warp_wait(pv_done(t, j - 1), p_parity(j - 1), abort);
                     if (!ok) break;
                 }
                 const bool dead = q > t_max || (a.window > 0 && q < walk.w_min && q >= a.sinks);
 #pragma unroll
                 for (int sp = 0; sp < SPT; ++sp) {
                     const int e = v_seq(j) + sp, s = e % NST;
-                    ok = ok && __all_sync(0xffffffffu, tc::wait_phase(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort));
+                    ok = ok && tc::warp_wait(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
                     if (!ok) break;
                     if (dead) {
                         uint4* row = reinterpret_cast<uint4*>(ring + s * C::kStage + (q - j0) * 128);
@@ -457,10 +433,44 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 if (!ok) break;
                 fence_proxy_async_smem();
             }
-            const float2 sc = make_float2(wk.scale2, wk.scale2), nm = make_float2(-m2, -m2);
-            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            const float2 sc = make_float2(wk.scale2, wk.scale2);
+            float2 sum[2];
             uint32_t p[kKeys / 4];
-            auto weights = [&](int q) {  // columns 32 q .. 32 q + 31
+            float m2 = m == -INFINITY ? 0.f : m * wk.scale2;
+            // The running maximum moves to the row's largest score so far.
+            auto raise = [&]() {
+                float top[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) top[q] = x[q];
+#pragma unroll
+                for (int c = 8; c < kKeys; ++c) top[c & 7] = fmaxf(top[c & 7], x[c]);
+#pragma unroll
+                for (int q = 4; q > 0; q >>= 1)
+#pragma unroll
+                    for (int i = 0; i < q; ++i) top[i] = fmaxf(top[i], top[i + q]);
+                const float mn = fmaxf(m, top[0]), f = m == -INFINITY ? 0.f : tc::ex2((m - mn) * wk.scale2);
+                m = mn;
+                m2 = m == -INFINITY ? 0.f : m * wk.scale2;
+                l *= f;
+                if (j == 0) return;
+                ok = tc::warp_wait(pv_done(t, j - 1), p_parity(j - 1), abort);
+                if (!ok) return;
+                tc::fence_after();
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    uint32_t u[32];
+                    tc::ld32(tmem + lanes + C::o_col(t) + c, o);
+                    tc::wait_ld();
+                    tc::tie32(o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * f);
+                    tc::st32(tmem + lanes + C::o_col(t) + c, u);
+                }
+                tc::wait_st();
+            };
+            auto weights = [&](int q) {  // of columns 32 q .. 32 q + 31
+                const float2 nm = make_float2(-m2, -m2);
 #pragma unroll
                 for (int c = 0; c < 32; c += 2) {
                     float2 w = ffma2(make_float2(x[32 * q + c], x[32 * q + c + 1]), sc, nm);
@@ -469,8 +479,31 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                     p[16 * (q & 1) + c / 2] = pack16(w.x, w.y, T());
                 }
             };
-            weights(0);
-            weights(1);
+            // The first half's weights are taken under the old maximum, and the
+            // maximum is raised (and they are taken again) only where their sum
+            // or a score of the second half asks for it: looking for the largest
+            // of 128 scores first costs 250 clocks a tile, the second half's
+            // search hides behind the exponentials.
+            const bool fresh = __any_sync(0xffffffffu, live && m == -INFINITY);
+            if (fresh) raise();
+            if (!ok) break;
+            auto first_half = [&]() -> bool {
+                sum[0] = sum[1] = make_float2(0.f, 0.f);
+                float top[4] = {x[64], x[65], x[66], x[67]};
+                weights(0);
+#pragma unroll
+                for (int c = 68; c < kKeys; ++c) top[c & 3] = fmaxf(top[c & 3], x[c]);
+                weights(1);
+                const float s = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                const float t2 = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                return s > kMaxWeight || fmaf(t2, wk.scale2, -m2) > kMaxSlack;
+            };
+            const bool over = first_half();
+            if (!fresh && __any_sync(0xffffffffu, over)) {
+                raise();
+                if (!ok) break;
+                (void)first_half();
+            }
             tc::st32(tmem + lanes + C::p_col(t, j), p);
             weights(2);
             tc::wait_st();
@@ -485,7 +518,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full(t, j));
         }
-        if (ok && nj > 0) ok = __all_sync(0xffffffffu, tc::wait_phase(pv_done(t, nj - 1), p_parity(nj - 1), abort));
+        if (ok && nj > 0) ok = tc::warp_wait(pv_done(t, nj - 1), p_parity(nj - 1), abort);
         if (!ok) tc::give_up(abort, a.err);
         tc::fence_after();
         constexpr int CS = D + 4;

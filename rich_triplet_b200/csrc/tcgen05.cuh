@@ -22,25 +22,40 @@ __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int n, bool b_mn) {
 // swizzle, 8-row groups 1024 bytes apart.  K contiguous: `addr` is the tile's
 // row 0 plus 32 bytes per 16-element slice; `lead` is not used.  N contiguous:
 // rows are steps of K, and `lead` is the distance of the next 64 elements of N.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lead) {
-    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(lead >> 4) << 16) |
-           (uint64_t{1024 >> 4} << 32) | (uint64_t{1} << 46) | (uint64_t{2} << 61);
+// The descriptor's low word moves with the address by `step` / 16, so a
+// product's descriptors are one word each plus constants.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lead) {
+    return ((addr & 0x3FFFFu) >> 4) | ((lead >> 4) << 16);
+}
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t lo, uint32_t step) {
+    constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    return static_cast<uint64_t>(lo + (step >> 4)) | (static_cast<uint64_t>(kHi) << 32);
+}
+// A value that is the same in every lane, in a form that the compiler knows to
+// be: what goes into descriptors then stays in uniform registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+    return p != 0;
 }
 
 // D (tensor memory) = A (shared memory) B, + D if `accumulate`.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 // The same with A in tensor memory: lane = row, a 32-bit column = two steps of K.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 
@@ -110,6 +125,12 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
             else if (t - t0 > 1000000000ull) return false;
         }
     }
+}
+
+// The same for a whole warp, with one answer (every lane polls: one lane polling
+// for all measured 10 % slower prompts).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    return __all_sync(0xffffffffu, wait_phase(bar, parity, abort)) != 0;
 }
 
 __device__ __forceinline__ void give_up(volatile int* abort, int* err) {
