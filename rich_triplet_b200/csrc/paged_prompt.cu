@@ -195,6 +195,10 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         fence_mbar_init();
     }
     if (warp == 0) tc::alloc(tmem_slot, 512);
+    if (warp == C::kSoftWarps && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
+    }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -352,19 +356,26 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // tensor-memory lane 32 (warp % 4), bits 16 on
         const int nj = tiles_of(t), n0 = tiles_of(0);
         {
-            // Q tile t into shared memory, rows past the end zero
-            constexpr int CPR = D / 8;  // 16-byte chunks of a row
-            uint8_t* qt = sm + t * C::kQTile;
-            for (int i = (warp & 3) * 32 + lane; i < kRows * CPR; i += 128) {
-                const int row = i / CPR, ch = i % CPR;
-                const int64_t rho = row0 + t * kRows + row;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (t * kRows + row < nrows) {
-                    const int64_t tok = rho / G;
-                    x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (q_first + tok) * a.q_row +
-                                                        (h * G + static_cast<int>(rho - tok * G)) * a.q_head + ch * 8);
+            // Q tile t into shared memory, rows past the end zero: a warp its own 32 rows
+            constexpr int CPR = D / 8, RPI = 32 / CPR;  // 16-byte chunks of a row; rows of a warp-wide load
+            const int own = r < nrows ? static_cast<int>((row0 + r) / G) : -1;  // this lane's row: its token
+            const int64_t off = own < 0 ? -1 : (q_first + own) * a.q_row + (h * G + static_cast<int>(row0 + r - static_cast<int64_t>(own) * G)) * a.q_head;
+            const int ch = lane % CPR;
+            uint8_t* dst = sm + t * C::kQTile + (ch >> 3) * C::kChunk + (warp & 3) * 32 * 128;
+#pragma unroll 1
+            for (int i0q = 0; i0q < 32; i0q += 8 * RPI) {
+                uint4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t o = __shfl_sync(0xffffffffu, off, i0q + i * RPI + lane / CPR);
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if (o >= 0) v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + o + ch * 8);
                 }
-                *reinterpret_cast<uint4*>(qt + (ch >> 3) * C::kChunk + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = x;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = i0q + i * RPI + lane / CPR;
+                    *reinterpret_cast<uint4*>(dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v[i];
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -376,6 +387,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         const int pos = live ? pos0 + tok : -1;
         const int tile_lo = pos0 + static_cast<int>((row0 + t * kRows) / G);
         const int tile_hi = pos0 + static_cast<int>((row0 + min(nrows, (t + 1) * kRows) - 1) / G);
+        const bool warp_live = t * kRows + (warp & 3) * 32 < nrows;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; j < nj; ++j) {
@@ -384,11 +396,13 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             if (!ok) break;
             tc::fence_after();
             float x[kKeys];
+            if (warp_live) {
 #pragma unroll
-            for (int c = 0; c < kKeys; c += 32) tc::ld32(tmem + lanes + C::s_col(t) + c, x + c);
-            tc::wait_ld();
+                for (int c = 0; c < kKeys; c += 32) tc::ld32(tmem + lanes + C::s_col(t) + c, x + c);
+                tc::wait_ld();
 #pragma unroll
-            for (int c = 0; c < kKeys; c += 32) tc::tie32(x + c);
+                for (int c = 0; c < kKeys; c += 32) tc::tie32(x + c);
+            }
             if (!C::kAlias) {
                 tc::fence_before();
                 __syncwarp();
@@ -402,7 +416,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 tc::fence_after();
             }
             const int j0 = walk.tile(i0 + j) * kKeys;
-            if (j0 + kKeys - 1 > tile_lo || nrows < (t + 1) * kRows || (a.window > 0 && j0 <= tile_hi - a.window)) {
+            if (warp_live && (j0 + kKeys - 1 > tile_lo || nrows < (t + 1) * kRows || (a.window > 0 && j0 <= tile_hi - a.window))) {
                 // visible: c <= hi, and c > lo or c < first
                 const int hi = pos - j0, lo = a.window > 0 ? pos - a.window - j0 : -1, first = a.window > 0 ? a.sinks - j0 : 0;
 #pragma unroll
@@ -432,6 +446,15 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 }
                 if (!ok) break;
                 fence_proxy_async_smem();
+            }
+            if (!warp_live) {  // nobody reads these rows' outputs: whatever P holds will do
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(p_half(t, j));
+                    mbar_arrive(p_full(t, j));
+                }
+                continue;
             }
             const float2 sc = make_float2(wk.scale2, wk.scale2);
             float2 sum[2];
@@ -527,7 +550,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         T* out = static_cast<T*>(a.out) + (q_first + tok) * a.out_row + head * a.out_head;
         const bool none = m == -INFINITY;
         const float inv = none ? 0.f : 1.f / l;
-        if (ok) {
+        if (ok && warp_live) {
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float o[32];
@@ -598,24 +621,37 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                             M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
-                for (int i = threadIdx.x; i < nrows * (D / 4); i += kSoft) {
-                    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
-                    const float* p = recs + static_cast<int64_t>(row) * CS + d;
-                    const float* f = wgt + row * (kMaxSplit + 1);
-                    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+                // eight float4 of the output a thread at a time, so that their loads overlap
+                constexpr int kBatch = 8;
+                const int quads = nrows * (D / 4);
+#pragma unroll 1
+                for (int i0q = threadIdx.x; i0q < quads; i0q += kSoft * kBatch) {
+                    float4 A[kBatch];
+#pragma unroll
+                    for (int q = 0; q < kBatch; ++q) A[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
                     for (int s = 0; s < ns; ++s) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(p + s * kNext));
-                        A.x += v.x * f[s];
-                        A.y += v.y * f[s];
-                        A.z += v.z * f[s];
-                        A.w += v.w * f[s];
+#pragma unroll
+                        for (int q = 0; q < kBatch; ++q) {
+                            const int i = min(i0q + q * kSoft, quads - 1), row = i / (D / 4);
+                            const float4 v = __ldcg(reinterpret_cast<const float4*>(recs + s * kNext + row * CS + (i % (D / 4)) * 4));
+                            const float f = wgt[row * (kMaxSplit + 1) + s];
+                            A[q].x += v.x * f;
+                            A[q].y += v.y * f;
+                            A[q].z += v.z * f;
+                            A[q].w += v.w * f;
+                        }
                     }
-                    const int64_t rr = row0 + row, tk = rr / G;
-                    const float iv = f[kMaxSplit];
-                    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (q_first + tk) * a.out_row +
-                                              (h * G + static_cast<int>(rr - tk * G)) * a.out_head + d) =
-                        make_uint2(pack16(A.x * iv, A.y * iv, T()), pack16(A.z * iv, A.w * iv, T()));
+#pragma unroll
+                    for (int q = 0; q < kBatch; ++q) {
+                        const int i = i0q + q * kSoft, row = i / (D / 4);
+                        if (i >= quads) continue;
+                        const int rr = static_cast<int>(row0) + row, tk = rr / G;
+                        const float iv = wgt[row * (kMaxSplit + 1) + kMaxSplit];
+                        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (q_first + tk) * a.out_row + (h * G + rr - tk * G) * a.out_head +
+                                                  (i % (D / 4)) * 4) =
+                            make_uint2(pack16(A[q].x * iv, A[q].y * iv, T()), pack16(A[q].z * iv, A[q].w * iv, T()));
+                    }
                 }
             }
         }
