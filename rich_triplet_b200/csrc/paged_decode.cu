@@ -46,6 +46,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kSlotBytes = 8192;  // K or V rows of a tile, head_dim 256
 constexpr int kRingBytes = 3 * kSlotBytes;  // per warp
 constexpr float kMaxSlack = 8.f;
+constexpr int kJoinBatch = 16;    // partial results whose loads overlap in a join
 
 template <typename T, int D, int NT>
 struct DecCfg {
@@ -55,13 +56,15 @@ struct DecCfg {
     static constexpr int kSlot = kRows * kRowBytes;
     static constexpr int NS = kRingBytes / kSlot;               // 3, 6 or 12
     static constexpr int kUnit = kRows * kWarps;
+    static constexpr int kWhole = 3 * 256 / D;                   // units that cost what a join does
     static constexpr int kQBytes = kF32 ? NT * (D / 8) * 32 * 16 : 0;  // f32: query fragments
     static constexpr int CS = D + 4;                            // floats of a combine row
     static constexpr int kCombBytes = kWarps * NT * 8 * CS * 4;
     static constexpr int kMain = kWarps * kRingBytes > kCombBytes ? kWarps * kRingBytes : kCombBytes;
     static constexpr int kOffQ = kMain;
     static constexpr int kOffMisc = kOffQ + kQBytes;            // m, l of every warp and column; block scan
-    static constexpr int kSmem = kOffMisc + kWarps * NT * 8 * 8 + 64;
+    static constexpr int kOffRows = kOffMisc + kWarps * NT * 8 * 8 + 64;  // [warp][16] byte offsets of a tile's rows
+    static constexpr int kSmem = kOffRows + kWarps * 16 * 8;
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
@@ -73,6 +76,9 @@ __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+__device__ __forceinline__ void cp16_all(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -81,6 +87,12 @@ __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
+__device__ __forceinline__ int64_t lds64(uint32_t a) {
+    int64_t v;
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts64(uint32_t a, int64_t v) { asm volatile("st.shared.b64 [%0], %1;" ::"r"(a), "l"(v) : "memory"); }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -112,10 +124,17 @@ __device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, ui
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// x = hi + lo up to 2^-23 |x|, both tf32.
+__device__ __forceinline__ void mma8_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// x = hi + lo with hi's 11 leading bits; the product reads 11 bits of lo, which
+// leaves out at most 2^-21 |x|.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+    hi = __float_as_uint(x) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
@@ -166,68 +185,95 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
     const uint32_t ring = smem_u32(smem) + warp * kRingBytes;
+    const uint32_t rows_at = smem_u32(smem) + C::kOffRows + warp * 16 * 8;
     float* comb = reinterpret_cast<float*>(smem);
     float2* ml = reinterpret_cast<float2*>(smem + C::kOffMisc);  // [warp][NT * 8]
     int* red = reinterpret_cast<int*>(smem + C::kOffMisc + kWarps * NT * 8 * 8);
     const int G = a.G;
 
     // ---- this CTA's share of the units ----
+    // Prefix sums over the sequences of (units of an item, items) in one word each half.
     const int chunk = (kv.nseq + kThreads - 1) / kThreads;
     const int sb0 = min(kv.nseq, static_cast<int>(threadIdx.x) * chunk), sb1 = min(kv.nseq, sb0 + chunk);
-    int mine = 0;
-    for (int b = sb0; b < sb1; ++b) mine += (visible(kv.len(b), a.window, a.sinks).n + UNIT - 1) / UNIT;
-    int x = mine;
+    int64_t mine = 0;
+    int longest = 0;
+    for (int b = sb0; b < sb1; ++b) {
+        const int n = (visible(kv.len(b), a.window, a.sinks).n + UNIT - 1) / UNIT;
+        if (n > 0) mine += (static_cast<int64_t>(1) << 40) + n;
+        longest = max(longest, n);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    int64_t x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
-    if (lane == 31) red[warp] = x;
+    int64_t* red64 = reinterpret_cast<int64_t*>(red);
+    if (lane == 31) red64[warp] = x;
+    if (lane == 0) red[12 + warp] = longest;
     __syncthreads();
-    int before = x - mine, all = 0;
+    int64_t before = x - mine, all = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += red[w];
-        all += red[w];
+        if (w < warp) before += red64[w];
+        all += red64[w];
+        longest = max(longest, red[12 + w]);
     }
-    // every CTA below `grid` has a unit at least
-    const int64_t U = static_cast<int64_t>(all) * kv.nkv, grid = min(static_cast<int64_t>(gridDim.x), U);
+    constexpr int64_t kUnits = (static_cast<int64_t>(1) << 40) - 1;
+    // Every CTA below `grid` has a unit at least.  Items stay whole, one to a
+    // CTA, where the longest of them is at most kWhole units more than an even
+    // share: a split item is drained, joined and followed by another's start,
+    // which takes about as long (64 windows of 1028 positions on 4 heads of 256:
+    // 51 us dealt evenly, WINDOW_US us whole).
+    const int64_t U = (all & kUnits) * kv.nkv, items = (all >> 40) * kv.nkv;
+    const bool by_item = items > 0 && items <= gridDim.x && longest <= U / min(static_cast<int64_t>(gridDim.x), U) + C::kWhole;
+    const int64_t grid = by_item ? items : min(static_cast<int64_t>(gridDim.x), U);
     const bool idle = blockIdx.x >= grid;
-    const int64_t u_begin = idle ? U : blockIdx.x * U / grid, u_end = idle ? U : (blockIdx.x + 1) * U / grid;
-    __syncthreads();
+    const int64_t u_begin = idle ? U : blockIdx.x * U / grid;
+    int64_t u_end = idle ? U : (blockIdx.x + 1) * U / grid;
     {
-        const int64_t lo = static_cast<int64_t>(before) * kv.nkv, hi = lo + static_cast<int64_t>(mine) * kv.nkv;
-        if (u_begin >= lo && u_begin < hi) {  // one thread at most
-            int64_t u = lo;
+        // the one thread whose sequences hold this CTA's first unit (or item) finds it
+        const int64_t at = by_item ? static_cast<int64_t>(blockIdx.x) : u_begin;
+        const int shift = by_item ? 40 : 0;
+        const int64_t lo = ((before >> shift) & kUnits) * kv.nkv, hi = lo + ((mine >> shift) & kUnits) * kv.nkv;
+        if (!idle && at >= lo && at < hi) {
+            int64_t u = (before & kUnits) * kv.nkv, v = lo;
             for (int b = sb0; b < sb1; ++b) {
-                const int64_t n = static_cast<int64_t>((visible(kv.len(b), a.window, a.sinks).n + UNIT - 1) / UNIT) * kv.nkv;
-                if (u_begin < u + n) {
-                    red[4] = b;
-                    *reinterpret_cast<int64_t*>(&red[6]) = u;
+                const int64_t n = (visible(kv.len(b), a.window, a.sinks).n + UNIT - 1) / UNIT;
+                const int64_t step = (by_item ? (n > 0) : n) * kv.nkv;
+                if (at < v + step) {
+                    red[8] = b;
+                    red[9] = static_cast<int>(by_item ? at - v : 0);
+                    red64[5] = u;
                     break;
                 }
-                u += n;
+                u += n * kv.nkv;
+                v += step;
             }
         }
     }
     // Sequences that see nothing: output 0, lse -inf.
-    for (int b = blockIdx.x; b < kv.nseq; b += gridDim.x) {
-        if (visible(kv.len(b), a.window, a.sinks).n > 0) continue;
-        for (int i = threadIdx.x; i < a.nq * D; i += kThreads)
-            static_cast<T*>(a.out)[b * a.out_row + (i / D) * a.out_head + i % D] = from_f32<T>(0.f);
-        for (int i = threadIdx.x; i < a.nq; i += kThreads)
-            if (a.lse) a.lse[b * a.lse_row + i] = -INFINITY;
-    }
-    __syncthreads();
+    if ((all >> 40) < kv.nseq)
+        for (int b = blockIdx.x; b < kv.nseq; b += gridDim.x) {
+            if (visible(kv.len(b), a.window, a.sinks).n > 0) continue;
+            for (int i = threadIdx.x; i < a.nq * D; i += kThreads)
+                static_cast<T*>(a.out)[b * a.out_row + (i / D) * a.out_head + i % D] = from_f32<T>(0.f);
+            for (int i = threadIdx.x; i < a.nq; i += kThreads)
+                if (a.lse) a.lse[b * a.lse_row + i] = -INFINITY;
+        }
     if (idle) return;
-    int b = red[4];
-    int64_t u_item = *reinterpret_cast<int64_t*>(&red[6]);  // first unit of (b, h)
+    __syncthreads();
+    int b = red[8];
+    int64_t u_item = red64[5];  // first unit of (b, h)
     Visible vis = visible(kv.len(b), a.window, a.sinks);
     int nun = (vis.n + UNIT - 1) / UNIT;  // units of an item of sequence b
-    int h = static_cast<int>((u_begin - u_item) / nun);
+    int h = by_item ? red[9] : static_cast<int>((u_begin - u_item) / nun);
     u_item += static_cast<int64_t>(h) * nun;
+    const int64_t u_first = by_item ? u_item : u_begin;
+    if (by_item) u_end = u_item + nun;
 
-    for (int64_t u = u_begin; u < u_end;) {
+    for (int64_t u = u_first; u < u_end;) {
         const int t0 = static_cast<int>(u - u_item), t1 = static_cast<int>(min(u_end - u_item, static_cast<int64_t>(nun)));
         const int c_end = min(vis.n, t1 * UNIT);
         const int c_first = t0 * UNIT + warp * ROWS;  // this warp's tiles: c_first, + UNIT, ...
@@ -236,28 +282,34 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
 
         // ---- copies: half-tile s = 2 i + (0: K, 1: V) of tile i to slot s % NS ----
         int issued = 0, islot = 0;
-        int64_t off = -1, off_next = -1;
+        bool whole_tile = true;
+        const char* const kl = static_cast<const char*>(kv.k) + hoff * sizeof(T) + (lane % CPR) * 16;
+        const char* const vl = static_cast<const char*>(kv.v) + hoff * sizeof(T) + (lane % CPR) * 16;
         auto row_of = [&](int i) -> int64_t {
             const int c = c_first + i * UNIT + (lane % ROWS);
             return i < tiles && c < c_end ? kv.row(b, vis.pos(c)) : -1;
         };
-        off_next = row_of(0);
+        int64_t off_next = row_of(0);
         auto issue = [&]() {
             const int half = issued & 1;
             if (half == 0) {
-                off = off_next;
+                __syncwarp();  // the last tile's offsets have been read
+                if (lane < ROWS) sts64(rows_at + lane * 8, off_next < 0 ? -1 : off_next * static_cast<int64_t>(sizeof(T)));
+                whole_tile = __all_sync(0xffffffffu, off_next >= 0);
                 off_next = row_of((issued >> 1) + 1);
             }
             if (issued < 2 * tiles) {
-                const char* base = static_cast<const char*>(half ? kv.v : kv.k) + hoff * sizeof(T);
+                const char* base = half ? vl : kl;
                 const uint32_t dst = ring + islot * C::kSlot;
 #pragma unroll
                 for (int i = 0; i < COPIES; ++i) {
-                    const int id = i * 32 + lane, r = id / CPR, ch = id % CPR;
-                    const int64_t o = __shfl_sync(0xffffffffu, off, r);
-                    const int sw = F32 ? 2 * (r & 3) + (r >> 2) : (r & 7);
-                    cp16(dst + r * C::kRowBytes + ((ch ^ sw) << 4), base + (o < 0 ? 0 : o) * static_cast<int64_t>(sizeof(T)) + ch * 16,
-                         o >= 0);
+                    // a warp-wide copy is 32 / CPR rows, or a part of one
+                    const int r = CPR >= 32 ? i / (CPR / 32) : i * (32 / CPR) + lane / CPR, part = CPR >= 32 ? i % (CPR / 32) : 0;
+                    const int sw = F32 ? 2 * (r & 3) + (r >> 2) : (r & 7), ch = part * 32 + lane % CPR;
+                    const uint32_t to = dst + r * C::kRowBytes + ((ch ^ sw) << 4);
+                    const int64_t o = lds64(rows_at + r * 8);
+                    if (whole_tile) cp16_all(to, base + o + part * 512);
+                    else cp16(to, base + (o < 0 ? 0 : o) + part * 512, o >= 0);
                 }
             }
             cp_commit();
@@ -319,7 +371,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
             const uint32_t ks = ring + slot * C::kSlot;
             if constexpr (!F32) {
                 const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
-                const uint32_t rb = ks + r * C::kRowBytes;
+                // chunk (2 k + lane / 16) ^ (r % 8): the swizzle only turns bits 0..2
+                uint32_t at[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) at[k] = ks + r * C::kRowBytes + (((2 * k + (lane >> 4)) ^ (r & 7)) << 4);
                 float acc[2][NT][4];
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
@@ -330,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
 #pragma unroll
                 for (int k = 0; k < KQ; ++k) {
                     uint32_t kf[4];
-                    ldsm4(rb + (((2 * k + (lane >> 4)) ^ (r & 7)) << 4), kf);
+                    ldsm4(at[k & 3] + (k >> 2) * 128, kf);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma16<T>(acc[k & 1][n], kf, qf[n][k][0], qf[n][k][1]);
                 }
@@ -341,8 +396,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
             } else {
                 const uint4* qs = reinterpret_cast<const uint4*>(smem + C::kOffQ) + lane;
                 const int r = lane & 7;
-                const uint32_t rb = ks + r * C::kRowBytes;
                 const int sw = 2 * (r & 3) + (r >> 2);
+                const uint32_t at[2] = {ks + r * C::kRowBytes + (((lane >> 3) ^ sw) << 4),
+                                        ks + r * C::kRowBytes + (((4 + (lane >> 3)) ^ sw) << 4)};
                 // The tensor cores' f32 sums cut off instead of rounding: four short
                 // chains for the large products, added here.
                 float hh[4][NT][4], lh[NT][4], hl[NT][4];
@@ -354,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
 #pragma unroll 4
                 for (int k2 = 0; k2 < D / 16; ++k2) {  // chain 2 (k2 % 2) + k of hh
                     uint32_t kf[4];
-                    ldsm4(rb + (((4 * k2 + (lane >> 3)) ^ sw) << 4), kf);
+                    ldsm4(at[k2 & 1] + (k2 >> 1) * 128, kf);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         uint32_t h0, h1, l0, l1;
@@ -439,11 +495,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                         }
                     }
                 const int mi = lane >> 3, r = (lane & 7) + (mi >> 1) * 8;
-                const uint32_t rb = vs + r * C::kRowBytes;
+                uint32_t at[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) at[j] = vs + r * C::kRowBytes + (((2 * j + (mi & 1)) ^ (r & 7)) << 4);
 #pragma unroll
                 for (int j = 0; j < MT; ++j) {
                     uint32_t vf[4];
-                    ldsm4t(rb + (((2 * j + (mi & 1)) ^ (r & 7)) << 4), vf);
+                    ldsm4t(at[j & 3] + (j >> 2) * 128, vf);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         mma16<T>(o[n][j], vf, hi[n][0], hi[n][1]);
@@ -460,19 +518,25 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                         const float p0 = __shfl_sync(0xffffffffu, s[n][0], src), p1 = __shfl_sync(0xffffffffu, s[n][1], src);
                         split_tf32((g8 & 1) ? p1 : p0, ph[n][q], pl[n][q]);
                     }
+                // value q of 16-dim tile j: dims 16 j + g8 + 8 (q & 1), positions t4 + 4 (q >> 1);
+                // its chunk 4 j + 2 (q & 1) + g8 / 4 is turned in bits 0..2 by the swizzle
+                uint32_t at[2][4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int r = t4 + 4 * (q >> 1), sw = 2 * (r & 3) + (r >> 2);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        at[j][q] = vs + r * C::kRowBytes + (((4 * j + 2 * (q & 1) + (g8 >> 2)) ^ sw) << 4) + (g8 & 3) * 4;
+                }
 #pragma unroll
                 for (int j = 0; j < MT; ++j) {
                     uint32_t vh[4], vl[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {  // rows (dims) g8, g8 + 8; positions t4, t4 + 4
-                        const int r = t4 + 4 * (q >> 1), d = 16 * j + g8 + 8 * (q & 1);
-                        const int sw = 2 * (r & 3) + (r >> 2);
-                        split_tf32(lds32(vs + r * C::kRowBytes + (((d >> 2) ^ sw) << 4) + (d & 3) * 4), vh[q], vl[q]);
-                    }
+                    for (int q = 0; q < 4; ++q) split_tf32(lds32(at[j & 1][q] + (j >> 1) * 128), vh[q], vl[q]);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        float z[4] = {0.f, 0.f, 0.f, 0.f};  // one tile's sum, added with rounding
-                        mma8(z, vh[0], vh[1], vh[2], vh[3], pl[n][0], pl[n][1]);
+                        float z[4];  // one tile's sum, added with rounding
+                        mma8_zero(z, vh[0], vh[1], vh[2], vh[3], pl[n][0], pl[n][1]);
                         mma8(z, vl[0], vl[1], vl[2], vl[3], ph[n][0], ph[n][1]);
                         mma8(z, vh[0], vh[1], vh[2], vh[3], ph[n][0], ph[n][1]);
 #pragma unroll
@@ -509,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
         __syncthreads();
         const bool whole = t0 == 0 && t1 == nun;
         const int64_t item_row = b;
-        const int rec = 2 * blockIdx.x + (u == u_begin ? 0 : 1);
+        const int rec = 2 * blockIdx.x + (u == u_first ? 0 : 1);
         float* pr = wk.part + static_cast<int64_t>(rec) * G * CS;
         for (int i = threadIdx.x; i < G * (D / 4); i += kThreads) {
             const int g = i / (D / 4), d = (i % (D / 4)) * 4;
@@ -566,34 +630,46 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                 // CTA c_a's part is its last segment, unless its share begins with the item
                 const int first = 2 * c_a + (c_a * U / grid == u_item ? 0 : 1);
                 auto record = [&](int k) { return wk.part + static_cast<int64_t>(k ? 2 * (c_a + k) : first) * G * CS; };
-                float* wgt = comb;  // [n][G] weights, then [G] sums and maxima
-                for (int g = threadIdx.x; g < G; g += kThreads) {
+                float2* st = reinterpret_cast<float2*>(smem);  // [n][G] maximum and sum, then weight and sum
+                for (int i = threadIdx.x; i < n * G; i += kThreads)
+                    st[i] = __ldcg(reinterpret_cast<const float2*>(record(i / G) + (i % G) * CS + D));
+                __syncthreads();
+                for (int g = warp; g < G; g += kWarps) {
                     float M = -INFINITY, L = 0.f;
-                    for (int k = 0; k < n; ++k) M = fmaxf(M, __ldcg(record(k) + g * CS + D));
-                    for (int k = 0; k < n; ++k) {
-                        const float f = rel2(__ldcg(record(k) + g * CS + D), M);
-                        wgt[k * G + g] = f;
-                        L += f * __ldcg(record(k) + g * CS + D + 1);
+                    for (int k = lane; k < n; k += 32) M = fmaxf(M, st[k * G + g].x);
+                    M = warp_max(M);
+                    for (int k = lane; k < n; k += 32) {
+                        const float f = rel2(st[k * G + g].x, M);
+                        L += f * st[k * G + g].y;
+                        st[k * G + g].x = f;
                     }
-                    wgt[n * G + g] = 1.f / L;
-                    const int head = h * G + g;
-                    if (a.lse) a.lse[item_row * a.lse_row + head] = (M + log2f(L)) * 0.693147180559945309f;
-                    if (wk.norm) wk.norm[item_row * a.nq + head] = make_float2(M, 1.f / L);
+                    L = warp_sum(L);
+                    if (lane == 0) {
+                        st[n * G + g].x = 1.f / L;
+                        const int head = h * G + g;
+                        if (a.lse) a.lse[item_row * a.lse_row + head] = (M + log2f(L)) * 0.693147180559945309f;
+                        if (wk.norm) wk.norm[item_row * a.nq + head] = make_float2(M, 1.f / L);
+                    }
                 }
                 __syncthreads();
                 for (int i = threadIdx.x; i < G * (D / 4); i += kThreads) {
                     const int g = i / (D / 4), d = (i % (D / 4)) * 4;
                     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                    for (int k = 0; k < n; ++k) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(record(k) + g * CS + d));
-                        const float f = wgt[k * G + g];
-                        A.x += v.x * f;
-                        A.y += v.y * f;
-                        A.z += v.z * f;
-                        A.w += v.w * f;
+                    for (int k0 = 0; k0 < n; k0 += kJoinBatch) {
+                        float4 v[kJoinBatch];
+#pragma unroll
+                        for (int k = 0; k < kJoinBatch; ++k)
+                            v[k] = __ldcg(reinterpret_cast<const float4*>(record(min(k0 + k, n - 1)) + g * CS + d));
+#pragma unroll
+                        for (int k = 0; k < kJoinBatch; ++k) {
+                            const float f = k0 + k < n ? st[(k0 + k) * G + g].x : 0.f;
+                            A.x += v[k].x * f;
+                            A.y += v[k].y * f;
+                            A.z += v[k].z * f;
+                            A.w += v[k].w * f;
+                        }
                     }
-                    const float inv = wgt[n * G + g];
+                    const float inv = st[n * G + g].x;
                     T* out = static_cast<T*>(a.out) + item_row * a.out_row + (h * G + g) * a.out_head + d;
                     store4(out, A, inv);
                 }
