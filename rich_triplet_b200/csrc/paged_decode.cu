@@ -33,6 +33,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "paged.cuh"
@@ -46,7 +47,6 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kSlotBytes = 8192;  // K or V rows of a tile, head_dim 256
 constexpr int kRingBytes = 3 * kSlotBytes;  // per warp
 constexpr float kMaxSlack = 8.f;
-constexpr int kJoinBatch = 16;    // partial results whose loads overlap in a join
 
 template <typename T, int D, int NT>
 struct DecCfg {
@@ -56,6 +56,9 @@ struct DecCfg {
     static constexpr int kSlot = kRows * kRowBytes;
     static constexpr int NS = kRingBytes / kSlot;               // 3, 6 or 12
     static constexpr int kUnit = kRows * kWarps;
+    // An item's start (page lookups, an empty ring, a combine at its end) takes
+    // about as long as kStart units; it is dealt out like units without rows.
+    static constexpr int kStart = 256 / D;
     static constexpr int kWhole = 3 * 256 / D;                   // units that cost what a join does
     static constexpr int kQBytes = kF32 ? NT * (D / 8) * 32 * 16 : 0;  // f32: query fragments
     static constexpr int CS = D + 4;                            // floats of a combine row
@@ -195,10 +198,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
     // Prefix sums over the sequences of (units of an item, items) in one word each half.
     const int chunk = (kv.nseq + kThreads - 1) / kThreads;
     const int sb0 = min(kv.nseq, static_cast<int>(threadIdx.x) * chunk), sb1 = min(kv.nseq, sb0 + chunk);
+    auto units_of = [](int seen) { return seen > 0 ? C::kStart + (seen + UNIT - 1) / UNIT : 0; };
+    auto item_units = [&](int b) { return units_of(visible(kv.len(b), a.window, a.sinks).n); };
     int64_t mine = 0;
     int longest = 0;
     for (int b = sb0; b < sb1; ++b) {
-        const int n = (visible(kv.len(b), a.window, a.sinks).n + UNIT - 1) / UNIT;
+        const int n = item_units(b);
         if (n > 0) mine += (static_cast<int64_t>(1) << 40) + n;
         longest = max(longest, n);
     }
@@ -240,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
         if (!idle && at >= lo && at < hi) {
             int64_t u = (before & kUnits) * kv.nkv, v = lo;
             for (int b = sb0; b < sb1; ++b) {
-                const int64_t n = (visible(kv.len(b), a.window, a.sinks).n + UNIT - 1) / UNIT;
+                const int64_t n = item_units(b);
                 const int64_t step = (by_item ? (n > 0) : n) * kv.nkv;
                 if (at < v + step) {
                     red[8] = b;
@@ -267,14 +272,20 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
     int b = red[8];
     int64_t u_item = red64[5];  // first unit of (b, h)
     Visible vis = visible(kv.len(b), a.window, a.sinks);
-    int nun = (vis.n + UNIT - 1) / UNIT;  // units of an item of sequence b
+    int nun = units_of(vis.n);  // units of an item of sequence b
     int h = by_item ? red[9] : static_cast<int>((u_begin - u_item) / nun);
     u_item += static_cast<int64_t>(h) * nun;
     const int64_t u_first = by_item ? u_item : u_begin;
     if (by_item) u_end = u_item + nun;
 
     for (int64_t u = u_first; u < u_end;) {
-        const int t0 = static_cast<int>(u - u_item), t1 = static_cast<int>(min(u_end - u_item, static_cast<int64_t>(nun)));
+        // units [t0, t1) of the item, less the ones that stand for its start
+        const int seg_end = static_cast<int>(min(u_end - u_item, static_cast<int64_t>(nun)));
+        const int t0 = max(0, static_cast<int>(u - u_item) - C::kStart), t1 = seg_end - C::kStart;
+        if (t1 <= t0) {  // nothing but (a part of) the start: the next CTA reads the rows
+            u = u_item + seg_end;
+            continue;
+        }
         const int c_end = min(vis.n, t1 * UNIT);
         const int c_first = t0 * UNIT + warp * ROWS;  // this warp's tiles: c_first, + UNIT, ...
         const int tiles = c_first < c_end ? (c_end - c_first + UNIT - 1) / UNIT : 0;
@@ -571,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
             }
         }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == nun;
+        const bool whole = t0 == 0 && seg_end == nun;
         const int64_t item_row = b;
         const int rec = 2 * blockIdx.x + (u == u_first ? 0 : 1);
         float* pr = wk.part + static_cast<int64_t>(rec) * G * CS;
@@ -615,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
         if (!whole) {
             // ---- the CTAs c_a .. c_z hold parts of this item; the last to arrive joins them in order ----
             const int64_t u_last = u_item + nun - 1;
-            const int c_a = static_cast<int>(((u_item + 1) * grid - 1) / U), c_z = static_cast<int>(((u_last + 1) * grid - 1) / U);
+            const int c_a = static_cast<int>(((u_item + C::kStart + 1) * grid - 1) / U), c_z = static_cast<int>(((u_last + 1) * grid - 1) / U);
             const int n = c_z - c_a + 1;
             __threadfence();
             __syncthreads();
@@ -627,8 +638,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
             __syncthreads();
             if (red[0]) {
                 __threadfence();
-                // CTA c_a's part is its last segment, unless its share begins with the item
-                const int first = 2 * c_a + (c_a * U / grid == u_item ? 0 : 1);
+                // CTA c_a's part is its last segment, unless its share begins in the item
+                const int first = 2 * c_a + (c_a * U / grid >= u_item ? 0 : 1);
                 auto record = [&](int k) { return wk.part + static_cast<int64_t>(k ? 2 * (c_a + k) : first) * G * CS; };
                 float2* st = reinterpret_cast<float2*>(smem);  // [n][G] maximum and sum, then weight and sum
                 for (int i = threadIdx.x; i < n * G; i += kThreads)
@@ -652,40 +663,46 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                     }
                 }
                 __syncthreads();
-                for (int i = threadIdx.x; i < G * (D / 4); i += kThreads) {
-                    const int g = i / (D / 4), d = (i % (D / 4)) * 4;
-                    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int k0 = 0; k0 < n; k0 += kJoinBatch) {
-                        float4 v[kJoinBatch];
+                // the loads of kBatch partial results overlap
+                auto add_up = [&](auto batch) {
+                    constexpr int kBatch = decltype(batch)::value;
+                    for (int i = threadIdx.x; i < G * (D / 4); i += kThreads) {
+                        const int g = i / (D / 4), d = (i % (D / 4)) * 4;
+                        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (int k0 = 0; k0 < n; k0 += kBatch) {
+                            float4 v[kBatch];
 #pragma unroll
-                        for (int k = 0; k < kJoinBatch; ++k)
-                            v[k] = __ldcg(reinterpret_cast<const float4*>(record(min(k0 + k, n - 1)) + g * CS + d));
+                            for (int k = 0; k < kBatch; ++k)
+                                v[k] = __ldcg(reinterpret_cast<const float4*>(record(min(k0 + k, n - 1)) + g * CS + d));
 #pragma unroll
-                        for (int k = 0; k < kJoinBatch; ++k) {
-                            const float f = k0 + k < n ? st[(k0 + k) * G + g].x : 0.f;
-                            A.x += v[k].x * f;
-                            A.y += v[k].y * f;
-                            A.z += v[k].z * f;
-                            A.w += v[k].w * f;
+                            for (int k = 0; k < kBatch; ++k) {
+                                const float f = k0 + k < n ? st[(k0 + k) * G + g].x : 0.f;
+                                A.x += v[k].x * f;
+                                A.y += v[k].y * f;
+                                A.z += v[k].z * f;
+                                A.w += v[k].w * f;
+                            }
                         }
+                        T* out = static_cast<T*>(a.out) + item_row * a.out_row + (h * G + g) * a.out_head + d;
+                        store4(out, A, st[n * G + g].x);
                     }
-                    const float inv = st[n * G + g].x;
-                    T* out = static_cast<T*>(a.out) + item_row * a.out_row + (h * G + g) * a.out_head + d;
-                    store4(out, A, inv);
-                }
+                };
+                if (n <= 4) add_up(std::integral_constant<int, 4>());
+                else if (n <= 8) add_up(std::integral_constant<int, 8>());
+                else add_up(std::integral_constant<int, 20>());
             }
         }
         __syncthreads();  // the combine area is free for the next segment's copies
 
-        u = u_item + t1;
-        if (t1 == nun) {  // next item: the next head, or the next sequence with something to see
+        u = u_item + seg_end;
+        if (seg_end == nun) {  // next item: the next head, or the next sequence with something to see
             u_item += nun;
             if (++h == kv.nkv && u < u_end) {
                 h = 0;
                 do {
                     vis = visible(kv.len(++b), a.window, a.sinks);
                 } while (vis.n == 0);
-                nun = (vis.n + UNIT - 1) / UNIT;
+                nun = units_of(vis.n);
             }
         }
     }
