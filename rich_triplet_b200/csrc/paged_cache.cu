@@ -79,23 +79,21 @@ cudaError_t append_to(const PagedKv& kv, const PagedRows& a, cudaStream_t s) {
 
 // ---- evict ----
 
-constexpr int kSelThreads = 1024;
-
+constexpr int kKeysEach = 8;                  // keys a thread holds of a block
+constexpr int kHeldBlocks = 4;                // blocks whose keys stay in registers
 constexpr uint32_t kLowestKey = 0x007FFFFFu;  // rank_key of -inf
+constexpr uint32_t kKeptKey = 0xFFFFFFFFu;    // rank_key of the ends that are always kept
 
-// Rank of a position as an unsigned number in the order of its mass: the kept
-// ends above everything, NaN and positions without a mass as -inf.  Adding 0
-// makes -0 and +0 equal.
-__device__ __forceinline__ uint32_t rank_key(const PagedEvict& e, const float* mass, int j, int len) {
-    if (j < e.sinks || j >= len - e.recent) return 0xFFFFFFFFu;
-    if (j >= e.mass_cap) return kLowestKey;
-    const float x = mass[j] + 0.f;
-    if (x != x) return kLowestKey;
-    const uint32_t u = __float_as_uint(x);
-    return (u >> 31) ? ~u : (u | 0x80000000u);
+// Rank of a position with mass x as an unsigned number in the order of x, NaN
+// as -inf; 0 past the end.  Adding 0 makes -0 and +0 equal.
+__device__ __forceinline__ uint32_t rank_key(const PagedEvict& e, float x, int j, int len) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    const uint32_t key = x != x ? kLowestKey : (u >> 31) ? ~u : (u | 0x80000000u);
+    return j >= len ? 0u : (j < e.sinks || j >= len - e.recent) ? kKeptKey : key;
 }
 
 // Exclusive prefix of `v` over the block's threads; `total` is the block's sum.
+template <int kThreads>
 __device__ __forceinline__ int block_prefix(int v, int* red, int& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int x = v;
@@ -107,7 +105,7 @@ __device__ __forceinline__ int block_prefix(int v, int* red, int& total) {
     __syncthreads();
     if (lane == 31) red[warp] = x;
     __syncthreads();
-    int w = lane < (blockDim.x >> 5) ? red[lane] : 0;
+    int w = lane < kThreads / 32 ? red[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, w, o);
@@ -118,86 +116,190 @@ __device__ __forceinline__ int block_prefix(int v, int* red, int& total) {
     return x - v + (warp ? before : 0);
 }
 
-// One CTA per (sequence, KV head): the budget-th largest key by four passes of
-// eight bits over the keys, then the kept positions in order.
-__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedKv kv, const PagedEvict e) {
-    __shared__ int hist[256];
+// One CTA per (sequence, KV head).  The keys are read once and stay in
+// registers where the cache holds at most kHeldBlocks blocks (HELD; else each
+// pass reads them again).  Three passes over 11, 11 and 10 bits find the key of
+// the last position kept, by a histogram in shared memory each; then the kept
+// positions are written in order: a warp owns 256 consecutive positions of a
+// block, so that ballots rank them inside the warp and one prefix over the
+// warps ranks the warps.  Latency-bound: 8192 positions of 128
+// rows in 10.7 us.
+template <int kThreads, bool HELD>
+__global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedKv kv, const PagedEvict e) {
+    __shared__ int hist[2048];
     __shared__ int red[32];
     __shared__ uint32_t s_prefix;
     __shared__ int s_want;
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    constexpr int kBlock = kThreads * kKeysEach;
+    pdl_launch_dependents();
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int len = kv.len(b), n = min(len, e.budget);
     const float* mass = e.mass + b * e.mass_seq + h * e.mass_head;
     float* mout = e.mass_out + b * e.mass_seq + h * e.mass_head;
     int32_t* kept = e.kept + (static_cast<int64_t>(b) * kv.nkv + h) * e.budget;
     if (h == 0 && tid == 0) e.new_lens[b] = n;
-    uint32_t prefix = 0;
-    int want = n;  // of the keys that share `prefix`, this many are kept
-    if (len > e.budget) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            for (int j = tid; j < len; j += kSelThreads) {
-                const uint32_t key = rank_key(e, mass, j, len);
-                if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255u], 1);
+    const int blocks = (len + kBlock - 1) / kBlock;
+    const bool all = len <= e.budget;
+    auto position = [&](int blk, int i) { return blk * kBlock + warp * 256 + i * 32 + lane; };
+    auto load_keys = [&](int blk, uint32_t(&k)[kKeysEach]) {  // all loads before the first use
+        float x[kKeysEach];
+#pragma unroll
+        for (int i = 0; i < kKeysEach; ++i) {
+            const int j = position(blk, i);
+            x[i] = j < len && j < e.mass_cap ? mass[j] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < kKeysEach; ++i) k[i] = rank_key(e, x[i], position(blk, i), len);
+    };
+    uint32_t held[HELD ? kHeldBlocks : 1][kKeysEach];
+    if (HELD) {
+#pragma unroll
+        for (int blk = 0; blk < kHeldBlocks; ++blk)
+            if (blk < blocks) load_keys(blk, held[HELD ? blk : 0]);
+    }
+    // f(block, its keys) for every block
+    auto for_blocks = [&](auto f) {
+        if (HELD) {
+#pragma unroll
+            for (int blk = 0; blk < kHeldBlocks; ++blk)
+                if (blk < blocks) f(blk, held[HELD ? blk : 0]);
+        } else {
+            for (int blk = 0; blk < blocks; ++blk) {
+                load_keys(blk, held[0]);
+                f(blk, held[0]);
             }
+        }
+    };
+    uint32_t last = 0;                       // key of the last position kept by rank
+    int want = n - e.sinks - e.recent;       // positions kept by rank; of those with key `last`, when it is known
+    if (!all && want == 0) last = kKeptKey - 1;  // above every mass
+    if (!all && want > 0) {
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+#pragma unroll
+            for (int i = tid; i < 2048; i += kThreads) hist[i] = 0;
             __syncthreads();
-            // thread t < 256 looks at digit 255 - t: the digit in which the count from above passes `want`
-            const int c = tid < 256 ? hist[255 - tid] : 0;
+            for_blocks([&](int, const uint32_t(&k)[kKeysEach]) {
+#pragma unroll
+                for (int i = 0; i < kKeysEach; ++i)
+                    if (k[i] != 0u && k[i] != kKeptKey &&
+                        (pass == 0 || (k[i] >> (pass == 1 ? 21 : 10)) == (last >> (pass == 1 ? 21 : 10))))
+                        atomicAdd(&hist[(k[i] >> shift) & (bins - 1)], 1);
+            });
+            __syncthreads();
+            // thread t looks at kDigits digits from the top: the one in which the count passes `want`
+            constexpr int kDigits = 2048 / kThreads;
+            const int top = bins - 1 - tid * kDigits;
+            int sum = 0;
+            if (top >= 0)
+#pragma unroll
+                for (int i = 0; i < kDigits; ++i) sum += hist[top - i];
             int total;
-            const int above = block_prefix(c, red, total);
-            if (tid < 256 && above < want && above + c >= want) {
-                s_prefix = prefix | (static_cast<uint32_t>(255 - tid) << shift);
-                s_want = want - above;
+            int above = block_prefix<kThreads>(sum, red, total);
+            if (above < want && above + sum >= want) {
+#pragma unroll
+                for (int i = 0; i < kDigits; ++i) {
+                    const int c = hist[top - i];
+                    if (above < want && above + c >= want) {
+                        s_prefix = last | static_cast<uint32_t>(top - i) << shift;
+                        s_want = want - above;
+                    }
+                    above += c;
+                }
             }
             __syncthreads();
-            prefix = s_prefix;
+            last = s_prefix;
             want = s_want;
             __syncthreads();
         }
     }
-    int done = 0, equal = 0;  // kept so far; keys equal to the threshold so far
-    for (int j0 = 0; j0 < len; j0 += kSelThreads) {
-        const int j = j0 + tid;
-        const uint32_t key = j < len ? rank_key(e, mass, j, len) : 0u;
-        bool keep = j < len;
-        if (len > e.budget) {
-            const bool eq = j < len && key == prefix;
-            int eqs;
-            const int eq_before = block_prefix(eq, red, eqs);
-            keep = j < len && (key > prefix || (eq && equal + eq_before < want));
-            equal += eqs;
+    int done = 0, equal = 0;  // kept so far; keys equal to `last` so far
+    const uint32_t below = (1u << lane) - 1u;
+    for_blocks([&](int blk, const uint32_t(&k)[kKeysEach]) {
+        uint32_t keep[kKeysEach];
+        int eq_base = 0;
+        if (!all) {
+            int eqs = 0;
+#pragma unroll
+            for (int i = 0; i < kKeysEach; ++i) eqs += __popc(__ballot_sync(0xffffffffu, k[i] == last));
+            int total;
+            // every lane adds its warp's count once: lane 0's carries it
+            const int before = block_prefix<kThreads>(lane == 0 ? eqs : 0, red, total);
+            eq_base = equal + __shfl_sync(0xffffffffu, before, 0);
+            equal += total;
         }
-        int kepts;
-        const int at = done + block_prefix(keep, red, kepts);
-        if (keep) {
-            kept[at] = j;
-            if (at < e.mass_cap) mout[at] = j < e.mass_cap ? mass[j] : 0.f;
+        int kepts = 0;
+#pragma unroll
+        for (int i = 0; i < kKeysEach; ++i) {
+            const uint32_t eq = __ballot_sync(0xffffffffu, !all && k[i] == last);
+            const bool mine = k[i] != 0u && (all || k[i] == kKeptKey || k[i] > last ||
+                                             (k[i] == last && eq_base + __popc(eq & below) < want));
+            eq_base += __popc(eq);
+            keep[i] = __ballot_sync(0xffffffffu, mine);
+            kepts += __popc(keep[i]);
         }
-        done += kepts;
-    }
-    for (int i = n + tid; i < e.budget; i += kSelThreads) kept[i] = -1;
-    for (int i = n + tid; i < e.mass_cap; i += kSelThreads) mout[i] = 0.f;
+        int total;
+        const int before = block_prefix<kThreads>(lane == 0 ? kepts : 0, red, total);
+        int at = done + __shfl_sync(0xffffffffu, before, 0);
+        done += total;
+#pragma unroll
+        for (int i = 0; i < kKeysEach; ++i) {
+            if (keep[i] >> lane & 1u) {
+                const int j = position(blk, i), to = at + __popc(keep[i] & below);
+                kept[to] = j;
+                if (to < e.mass_cap) mout[to] = j < e.mass_cap ? mass[j] : 0.f;
+            }
+            at += __popc(keep[i]);
+        }
+    });
+    for (int i = n + tid; i < e.budget; i += kThreads) kept[i] = -1;
+    for (int i = n + tid; i < e.mass_cap; i += kThreads) mout[i] = 0.f;
 }
 
-// One warp per kept row: its K and V to slot i of the destination pages.
-__global__ void __launch_bounds__(256) paged_gather_kernel(const PagedKv kv, const PagedEvict e, int esize) {
-    const int i = blockIdx.x * 8 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
-    if (i >= min(kv.len(b), e.budget)) return;
-    const int j = e.kept[(static_cast<int64_t>(b) * kv.nkv + h) * e.budget + i];
-    const int64_t src = kv.row(b, j);
-    const int32_t p = e.dst[b * e.dst_stride + (i >> kv.page_log2)];
-    if (static_cast<uint32_t>(p) >= static_cast<uint64_t>(kv.num_pages)) return;
-    const int64_t dst = p * kv.page_stride + (i & ((1 << kv.page_log2) - 1)) * kv.slot_stride;
-    const int words = kv.D * esize / 16;
-    for (int w = lane; w < words; w += 32) {
-        uint4 x = make_uint4(0, 0, 0, 0), y = x;
-        if (src >= 0) {
-            x = reinterpret_cast<const uint4*>(static_cast<const char*>(kv.k) + (src + h * kv.head_stride) * esize)[w];
-            y = reinterpret_cast<const uint4*>(static_cast<const char*>(kv.v) + (src + h * kv.head_stride) * esize)[w];
+// A warp moves the K and V of eight kept rows (row bytes 16 CPR), their page
+// lookups and then their loads in flight together: HBM-bound, kept rows read
+// and written once (32 x 4 x 2048 rows of 512 bytes, K and V: 94 us, 5.7 TB/s).
+template <int CPR>
+__global__ void __launch_bounds__(256) paged_gather_kernel(const PagedKv kv, const PagedEvict e) {
+    constexpr int kRows = 8, kEach = kRows * CPR / 32, kBatch = kEach < 8 ? kEach : 8;
+    const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
+    const int first = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kRows;
+    const int n = min(kv.len(b), e.budget);
+    pdl_wait();
+    if (first >= n) return;
+    const int64_t es = kv.type == kPagedF32 ? 4 : 2;
+    int64_t src = -1, dst = -1;  // byte offsets of row `first + lane`
+    const int i = first + lane;
+    if (lane < kRows && i < n) {
+        const int32_t p = e.dst[b * e.dst_stride + (i >> kv.page_log2)];
+        const int64_t s = kv.row(b, e.kept[(static_cast<int64_t>(b) * kv.nkv + h) * e.budget + i]);
+        if (s >= 0) src = (s + h * kv.head_stride) * es;
+        if (static_cast<uint32_t>(p) < static_cast<uint64_t>(kv.num_pages))
+            dst = (p * kv.page_stride + (i & ((1 << kv.page_log2) - 1)) * kv.slot_stride + h * kv.head_stride) * es;
+    }
+#pragma unroll
+    for (int x0 = 0; x0 < kEach; x0 += kBatch) {
+        uint4 k[kBatch], v[kBatch];
+        int64_t to[kBatch];
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+            const int id = (x0 + x) * 32 + lane, r = id / CPR, at = (id % CPR) * 16;
+            const int64_t s = __shfl_sync(0xffffffffu, src, r);
+            to[x] = __shfl_sync(0xffffffffu, dst, r);
+            if (to[x] >= 0) to[x] += at;
+            k[x] = v[x] = make_uint4(0, 0, 0, 0);
+            if (s >= 0) {
+                k[x] = *reinterpret_cast<const uint4*>(static_cast<const char*>(kv.k) + s + at);
+                v[x] = *reinterpret_cast<const uint4*>(static_cast<const char*>(kv.v) + s + at);
+            }
         }
-        reinterpret_cast<uint4*>(static_cast<char*>(kv.k) + (dst + h * kv.head_stride) * esize)[w] = x;
-        reinterpret_cast<uint4*>(static_cast<char*>(kv.v) + (dst + h * kv.head_stride) * esize)[w] = y;
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x)
+            if (to[x] >= 0) {
+                *reinterpret_cast<uint4*>(static_cast<char*>(kv.k) + to[x]) = k[x];
+                *reinterpret_cast<uint4*>(static_cast<char*>(kv.v) + to[x]) = v[x];
+            }
     }
 }
 
@@ -209,11 +311,23 @@ cudaError_t paged_append_launch(const PagedKv& kv, const PagedRows& r, cudaStrea
 }
 
 cudaError_t paged_evict_launch(const PagedKv& kv, const PagedEvict& e, cudaStream_t s) {
-    paged_select_kernel<<<dim3(kv.nkv, kv.nseq), kSelThreads, 0, s>>>(kv, e);
-    cudaError_t err = cudaGetLastError();
+    const dim3 rows(kv.nkv, kv.nseq);
+    // A small block's barriers cost less, a large one's threads hold fewer keys
+    // each: 700 positions take 7.1 us in 256 threads and 9.2 in 1024, 8192 take
+    // 17.4 and 10.7.
+    const int64_t cap = static_cast<int64_t>(kv.width) << kv.page_log2;
+    if (cap <= 256 * kKeysEach) paged_select_kernel<256, true><<<rows, 256, 0, s>>>(kv, e);
+    else if (cap <= kHeldBlocks * 1024 * kKeysEach) paged_select_kernel<1024, true><<<rows, 1024, 0, s>>>(kv, e);
+    else paged_select_kernel<1024, false><<<rows, 1024, 0, s>>>(kv, e);
+    const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
-    paged_gather_kernel<<<dim3((e.budget + 7) / 8, kv.nkv, kv.nseq), 256, 0, s>>>(kv, e, kv.type == kPagedF32 ? 4 : 2);
-    return cudaGetLastError();
+    const dim3 grid((e.budget + 63) / 64, kv.nkv, kv.nseq);
+    switch (kv.D * (kv.type == kPagedF32 ? 4 : 2) / 16) {
+        case 8: return rt_launch(paged_gather_kernel<8>, grid, 256, 0, s, true, kv, e);
+        case 16: return rt_launch(paged_gather_kernel<16>, grid, 256, 0, s, true, kv, e);
+        case 32: return rt_launch(paged_gather_kernel<32>, grid, 256, 0, s, true, kv, e);
+        default: return rt_launch(paged_gather_kernel<64>, grid, 256, 0, s, true, kv, e);
+    }
 }
 
 }  // namespace rt

@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
     // CTA, where the longest of them is at most kWhole units more than an even
     // share: a split item is drained, joined and followed by another's start,
     // which takes about as long (64 windows of 1028 positions on 4 heads of 256:
-    // 51 us dealt evenly, WINDOW_US us whole).
+    // 51 us dealt evenly, 46 us whole).
     const int64_t U = (all & kUnits) * kv.nkv, items = (all >> 40) * kv.nkv;
     const bool by_item = items > 0 && items <= gridDim.x && longest <= U / min(static_cast<int64_t>(gridDim.x), U) + C::kWhole;
     const int64_t grid = by_item ? items : min(static_cast<int64_t>(gridDim.x), U);
@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
             for (int i = threadIdx.x; i < a.nq; i += kThreads)
                 if (a.lse) a.lse[b * a.lse_row + i] = -INFINITY;
         }
+    pdl_launch_dependents();
     if (idle) return;
     __syncthreads();
     int b = red[8];
@@ -711,6 +712,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
 // mass[b][h][j] += the position's weights over the G heads, from the stored scores.
 __global__ void __launch_bounds__(256) paged_decode_mass_kernel(const PagedKv kv, const PagedAttn a, const DecWork wk) {
     const int c = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, b = blockIdx.z;
+    pdl_wait();
     const Visible vis = visible(kv.len(b), a.window, a.sinks);
     if (c >= vis.n) return;
     const int j = vis.pos(c);
@@ -796,8 +798,7 @@ cudaError_t paged_decode_launch(const PagedKv& kv, const PagedAttn& a, void* wor
     int64_t n = wk.score_stride;
     if (a.window > 0) n = std::min<int64_t>(n, static_cast<int64_t>(a.window) + a.sinks);
     if (n == 0) return cudaSuccess;
-    paged_decode_mass_kernel<<<dim3(static_cast<unsigned>((n + 255) / 256), kv.nkv, kv.nseq), 256, 0, s>>>(kv, a, wk);
-    return cudaGetLastError();
+    return rt_launch(paged_decode_mass_kernel, dim3(static_cast<unsigned>((n + 255) / 256), kv.nkv, kv.nseq), 256, 0, s, true, kv, a, wk);
 }
 
 }  // namespace rt
