@@ -10,9 +10,12 @@
 //
 // A CTA takes one tile of 128 positions of a (sequence, KV head), keeps its
 // keys in shared memory and walks the (token, head) rows that see it, 128 at a
-// time: a loading warpgroup gathers the query rows with cp.async into the
-// 128-byte-swizzled ring, the MMA thread forms the scores in one of four
-// tensor-memory buffers, and two warpgroups take alternate tiles.  Tiles of
+// time: the query rows come into a 128-byte-swizzled ring, the MMA thread forms
+// the scores in one of four tensor-memory buffers, and two warpgroups take
+// alternate tiles.  Where 128 is a multiple of G a tile's rows are one box of a
+// (column, head, token) tensor per 64 columns, which TMA fetches; for other G a
+// warpgroup gathers them with cp.async (its address arithmetic doubles a
+// tile's time at head_dim 256).  Tiles of
 // early positions, which most rows see, start first.
 //
 // With a window, the tiles of the first tokens are seen by every row and the
@@ -26,6 +29,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "gemv.cuh"
 #include "paged.cuh"
 #include "tcgen05.cuh"
 
@@ -53,10 +57,13 @@ template <int D>
 struct MCfg {
     static constexpr int kChunk = kTile * 128;  // 64 columns of 128 rows
     static constexpr int kOperand = (D / 64) * kChunk;
-    static constexpr int NST = D == 256 ? 2 : 4;
+    static constexpr int SPT = D == 256 ? 2 : 1;                  // ring stages of a query tile
+    static constexpr int SD = D / SPT;                            // columns of a stage
+    static constexpr int kStage = (SD / 64) * kChunk;
+    static constexpr int NST = D == 256 ? 4 : D == 128 ? 5 : 8;
     static constexpr int kOffRing = kOperand;
-    static constexpr int kOffRow = kOffRing + NST * kOperand;  // [adding warp][128] {log-sum, token position}
-    static constexpr int kOffTotal = kOffRow + kSumGroups * 4 * kTile * 8;  // [128] the second group's totals
+    static constexpr int kOffRow = kOffRing + NST * kStage;  // [adding warp][128] - log-sums of the tile's rows
+    static constexpr int kOffTotal = kOffRow + kSumGroups * 4 * kTile * 4;  // [128] the second group's totals
     static constexpr int kOffBar = kOffTotal + kTile * 4;
     static constexpr int kBars = 2 * NST + 2 * kBufs + 2;
     static constexpr int kOffMisc = kOffBar + kBars * 8;
@@ -64,11 +71,11 @@ struct MCfg {
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-template <typename T, int D>
+template <typename T, int D, bool TMAQ>
 __global__ void __launch_bounds__(kThreads, 1)
-    paged_prompt_mass_kernel(const __grid_constant__ CUtensorMap tm_k, const PagedKv kv, const PagedAttn a, const MassWork wk) {
+    paged_prompt_mass_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_q, const PagedKv kv, const PagedAttn a, const MassWork wk) {
     using C = MCfg<D>;
-    constexpr int NST = C::NST;
+    constexpr int NST = C::NST, SPT = C::SPT;
     constexpr bool BF16 = !std::is_same<T, __half>::value;
     extern __shared__ uint8_t smem_raw[];
 
@@ -122,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tid = threadIdx.x & 127;
     if (threadIdx.x == 0) {
         for (int s = 0; s < NST; ++s) {
-            mbar_init(&full[s], 4);
+            mbar_init(&full[s], TMAQ ? 1 : 4);
             mbar_init(&empty[s], 1);
         }
         for (int s = 0; s < kBufs; ++s) {
@@ -158,23 +165,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t kId = tc::idesc_f16(BF16, kTile, false);
         bool ok = tc::warp_wait(k_full, 0u, abort);
         for (int i = 0; i < n && ok; ++i) {
-            const int s = i % NST, buf = i % kBufs;
-            ok = tc::warp_wait(&full[s], static_cast<uint32_t>(i / NST) & 1u, abort) &&
-                 (i < kBufs || tc::warp_wait(&s_free[buf], static_cast<uint32_t>(i / kBufs - 1) & 1u, abort));
-            if (!ok) break;
-            tc::fence_after();
-            const uint32_t kb = tc::uniform(tc::desc_lo(smem_u32(sm), 16)), st = tc::uniform(tmem + buf * kTile);
-            const uint32_t qb = tc::uniform(tc::desc_lo(smem_u32(ring + s * C::kOperand), 16));
-            if (tc::elect()) {
+            const int buf = i % kBufs;
+            ok = i < kBufs || tc::warp_wait(&s_free[buf], static_cast<uint32_t>(i / kBufs - 1) & 1u, abort);
+            const uint32_t st = tc::uniform(tmem + buf * kTile);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t at = (k >> 2) * C::kChunk + (k & 3) * 32;
-                    tc::mma_ss(st, tc::desc_sw128(kb, at), tc::desc_sw128(qb, at), kId, k > 0);
+            for (int sp = 0; sp < SPT; ++sp) {
+                const int e = i * SPT + sp, s = e % NST;
+                ok = ok && tc::warp_wait(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
+                if (!ok) break;
+                tc::fence_after();
+                const uint32_t kb = tc::uniform(tc::desc_lo(smem_u32(sm) + sp * C::kStage, 16));
+                const uint32_t qb = tc::uniform(tc::desc_lo(smem_u32(ring + s * C::kStage), 16));
+                if (tc::elect()) {
+#pragma unroll
+                    for (int k = 0; k < C::SD / 16; ++k) {
+                        const uint32_t at = (k >> 2) * C::kChunk + (k & 3) * 32;
+                        tc::mma_ss(st, tc::desc_sw128(kb, at), tc::desc_sw128(qb, at), kId, sp > 0 || k > 0);
+                    }
+                    tc::commit(&empty[s]);
+                    if (sp == SPT - 1) tc::commit(&s_full[buf]);
                 }
-                tc::commit(&empty[s]);
-                tc::commit(&s_full[buf]);
+                __syncwarp();
             }
-            __syncwarp();
         }
         if (!ok) tc::give_up(abort, a.err);
         if (tc::elect()) tc::commit(drain);
@@ -183,100 +195,128 @@ __global__ void __launch_bounds__(kThreads, 1)
         (void)mbar_wait_timed(k_full, 0u);
         __syncwarp();
     } else if (warp >= kSumGroups * 4) {
-        // ---- query rows into the ring, one tile ahead of the one that is handed over ----
-        constexpr int CPR = D / 8;          // 16-byte chunks of a row
-        constexpr int RPI = 32 / CPR;       // rows of a warp-wide copy
-        const int row0 = (warp & 3) * 32;   // this warp's rows of a tile
+        // ---- query rows into the ring ----
         bool ok = true;
-        for (int i = 0; i <= n; ++i) {
-            if (i < n) {
-                const int s = i % NST;
-                ok = ok && (i < NST || tc::warp_wait(&empty[s], static_cast<uint32_t>(i / NST - 1) & 1u, abort));
-                if (!ok) break;
-                // rows past the end repeat the last one (their weight is 0)
-                const int rho = min(r_begin + i * kTile + row0 + lane, r_end - 1), tok = rho / G;
-                const int64_t off = (q_first + tok) * a.q_row + (h * G + rho - tok * G) * a.q_head;
-                const int ch = lane % CPR;
-                const T* src = static_cast<const T*>(a.q) + ch * 8;
-                const uint32_t dst = smem_u32(ring + s * C::kOperand) + (ch >> 3) * C::kChunk;
+        if constexpr (TMAQ) {
+            if (warp == kSumGroups * 4 && lane == 0) {
+                int done = 0;
+                for (int e = 0; e < n * SPT && ok; ++e) {
+                    const int s = e % NST;
+                    ok = e < NST || tc::wait_phase(&empty[s], static_cast<uint32_t>(e / NST - 1) & 1u, abort);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(&full[s], C::kStage);
+                    const int tok = (r_begin + (e / SPT) * kTile) / G;  // tiles begin with a token
+#pragma unroll
+                    for (int c = 0; c < C::SD / 64; ++c)
+                        tc::tma_3d(ring + s * C::kStage + c * C::kChunk, &tm_q, (e % SPT) * C::SD + 64 * c, h * G,
+                                   static_cast<int>(q_first) + tok, &full[s]);
+                    ++done;
+                }
+                // no copy may still be landing when the CTA exits
+                for (int e = max(0, done - NST); e < done; ++e)
+                    (void)mbar_wait_timed(&full[e % NST], static_cast<uint32_t>(e / NST) & 1u);
+            }
+            __syncwarp();
+        } else {
+            // gathered, one stage ahead of the one that is handed over
+            constexpr int CPR = C::SD / 8;      // 16-byte chunks of a row of a stage
+            constexpr int RPI = 32 / CPR;       // rows of a warp-wide copy
+            const int row0 = (warp & 3) * 32;   // this warp's rows of a tile
+            for (int e = 0; e <= n * SPT; ++e) {
+                if (e < n * SPT) {
+                    const int s = e % NST;
+                    ok = ok && (e < NST || tc::warp_wait(&empty[s], static_cast<uint32_t>(e / NST - 1) & 1u, abort));
+                    if (!ok) break;
+                    // rows past the end repeat the last one (their weight is 0)
+                    const int rho = min(r_begin + (e / SPT) * kTile + row0 + lane, r_end - 1), tok = rho / G;
+                    const int64_t off = (q_first + tok) * a.q_row + (h * G + rho - tok * G) * a.q_head;
+                    const int ch = lane % CPR;
+                    const T* src = static_cast<const T*>(a.q) + (e % SPT) * C::SD + ch * 8;
+                    const uint32_t dst = smem_u32(ring + s * C::kStage) + (ch >> 3) * C::kChunk;
 #pragma unroll 8
-                for (int x = 0; x < 32 / RPI; ++x) {
-                    const int r = x * RPI + lane / CPR, row = row0 + r;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4)),
-                                 "l"(src + __shfl_sync(0xffffffffu, off, r))
-                                 : "memory");
+                    for (int x = 0; x < 32 / RPI; ++x) {
+                        const int r = x * RPI + lane / CPR, row = row0 + r;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4)),
+                                     "l"(src + __shfl_sync(0xffffffffu, off, r))
+                                     : "memory");
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (e > 0) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[(e - 1) % NST]);
                 }
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (i > 0) {
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[(i - 1) % NST]);
-            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
         if (!ok) tc::give_up(abort, a.err);
     } else {
         // ---- thread = position ----
         const int grp = warp >> 2, j = j0 + (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
-        // a warp's own copy of the tile's rows: log-sum (powers of two; +inf for
-        // none, whose weight is then 0) and position
-        float2* rb = reinterpret_cast<float2*>(sm + C::kOffRow) + warp * kTile;
-        float2 next[4];
+        // a warp's own copy of the tile's rows: minus the log-sum (powers of two;
+        // -inf for none, whose weight is then 0)
+        float* rz = reinterpret_cast<float*>(sm + C::kOffRow) + warp * kTile;
+        float next_z[4];
         auto load_rows = [&](int i) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int rho = r_begin + i * kTile + lane + 32 * e, tok = rho / G;
-                next[e] = make_float2(INFINITY, 0.f);
-                if (i >= n || rho >= r_end) continue;
-                const float z = a.lse[(q_first + tok) * a.lse_row + h * G + rho - tok * G];
-                next[e] = make_float2(z == -INFINITY ? INFINITY : z * 1.44269504088896341f, __int_as_float(pos0 + tok));
+                const int rho = min(r_begin + i * kTile + lane + 32 * e, r_end - 1), tok = rho / G;
+                next_z[e] = a.lse[(q_first + tok) * a.lse_row + h * G + rho - tok * G];
             }
         };
+        // rows of the tokens that see position j: [see, until)
+        const int see = max(0, (j - pos0) * G);
+        const int until = a.window > 0 && j >= a.sinks
+                              ? static_cast<int>(min(static_cast<int64_t>(r_end), (static_cast<int64_t>(j) + a.window - pos0) * G)) : r_end;
         load_rows(grp);
         bool ok = true;
         for (int i = grp; i < n; i += kSumGroups) {
             __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) rb[lane + 32 * e] = next[e];
+            for (int e = 0; e < 4; ++e) rz[lane + 32 * e] = next_z[e] == -INFINITY ? -INFINITY : next_z[e] * -1.44269504088896341f;
             __syncwarp();
-            load_rows(i + kSumGroups);
+            if (i + kSumGroups < n) load_rows(i + kSumGroups);
             const int buf = i % kBufs;
             ok = tc::warp_wait(&s_full[buf], static_cast<uint32_t>(i / kBufs) & 1u, abort);
             if (!ok) break;
             tc::fence_after();
-            const int r0 = r_begin + i * kTile, r1 = min(r0 + kTile, r_end) - 1;
-            const int t_lo = pos0 + r0 / G, t_hi = pos0 + r1 / G;
-            const bool masked = j0 + kTile - 1 > t_lo || (a.window > 0 && j0 <= t_hi - a.window);
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            const int r0 = r_begin + i * kTile;
+            // columns [c_see, c_until) of this tile are rows that see position j
+            const int c_see = see - r0, c_until = until - r0;
+            const bool masked = __any_sync(0xffffffffu, c_see > 0 || c_until < kTile);
+            const float2 sc = make_float2(wk.scale2, wk.scale2);
+            float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
-            for (int c = 0; c < kTile; c += 32) {
-                float x[32];
+            for (int c = 0; c < kTile; c += 64) {
+                float x[64];
                 tc::ld32(tmem + lanes + buf * kTile + c, x);
+                tc::ld32(tmem + lanes + buf * kTile + c + 32, x + 32);
                 tc::wait_ld();
                 tc::tie32(x);
-                if (c == kTile - 32) {
+                tc::tie32(x + 32);
+                if (c > 0) {
                     tc::fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[buf]);
                 }
                 if (masked) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int t = __float_as_int(rb[c + e].y);
-                        if (j > t || (a.window > 0 && j <= t - a.window && j >= a.sinks)) x[e] = -INFINITY;
-                    }
+                    for (int e = 0; e < 64; ++e)
+                        if (c + e < c_see || c + e >= c_until) x[e] = -INFINITY;
                 }
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const float4 z = *reinterpret_cast<const float4*>(&rb[c + e]);
-                    part[e & 2] += tc::ex2(fmaf(x[e], wk.scale2, -z.x));
-                    part[(e & 2) + 1] += tc::ex2(fmaf(x[e + 1], wk.scale2, -z.z));
+                for (int e = 0; e < 64; e += 4) {
+                    const float4 z = *reinterpret_cast<const float4*>(rz + c + e);
+                    const float2 w0 = ffma2(make_float2(x[e], x[e + 1]), sc, make_float2(z.x, z.y));
+                    const float2 w1 = ffma2(make_float2(x[e + 2], x[e + 3]), sc, make_float2(z.z, z.w));
+                    part[0] = tc::add2(part[0], make_float2(tc::ex2(w0.x), tc::ex2(w0.y)));
+                    part[1] = tc::add2(part[1], make_float2(tc::ex2(w1.x), tc::ex2(w1.y)));
                 }
             }
-            total += (part[0] + part[1]) + (part[2] + part[3]);
+            total += (part[0].x + part[0].y) + (part[1].x + part[1].y);
         }
         if (!ok) tc::give_up(abort, a.err);
         if (grp == 1) reinterpret_cast<float*>(sm + C::kOffTotal)[tid] = total;
@@ -312,10 +352,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-template <typename T, int D>
-cudaError_t launch(const PagedKv& kv, const PagedAttn& a, MassWork wk, int num_sms, cudaStream_t s) {
+// The queries as a 3-D tensor (column, head, token); boxes of 128 / G tokens x
+// G heads x 64 columns.  False where there is no such map.
+bool query_map(const PagedKv& kv, const PagedAttn& a, CUtensorMap* out) {
+    const TmapEncodeFn encode = tmap_encoder();
+    if (!encode || kTile % a.G != 0 || a.q_row == 0 || (a.nq > 1 && a.q_head == 0)) return false;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(kv.D), static_cast<cuuint64_t>(a.nq), static_cast<cuuint64_t>(a.rows)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.nq > 1 ? a.q_head : kv.D) * 2, static_cast<cuuint64_t>(a.q_row) * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.G), static_cast<cuuint32_t>(kTile / a.G)}, estr[3] = {1, 1, 1};
+    return encode(out, kv.type == kPagedF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                  const_cast<void*>(a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D, bool TMAQ>
+cudaError_t launch(const PagedKv& kv, const PagedAttn& a, const CUtensorMap& tq, MassWork wk, int num_sms, cudaStream_t s) {
     using C = MCfg<D>;
-    auto kernel = paged_prompt_mass_kernel<T, D>;
+    auto kernel = paged_prompt_mass_kernel<T, D, TMAQ>;
     static bool done[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -338,15 +391,21 @@ cudaError_t launch(const PagedKv& kv, const PagedAttn& a, MassWork wk, int num_s
     wk.first_parts = wk.first_items > 0 ? std::max(wk.parts, share(wk.first_items)) : 1;
     const int64_t grid = wk.first_items * wk.first_parts + (items - wk.first_items) * wk.parts;
     if (grid > INT32_MAX) return cudaErrorInvalidValue;
-    kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmem, s>>>(tk, kv, a, wk);
+    kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmem, s>>>(tk, tq, kv, a, wk);
     return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t by_dim(const PagedKv& kv, const PagedAttn& a, const MassWork& wk, int num_sms, cudaStream_t s) {
-    if (kv.D == 64) return launch<T, 64>(kv, a, wk, num_sms, s);
-    if (kv.D == 128) return launch<T, 128>(kv, a, wk, num_sms, s);
-    return launch<T, 256>(kv, a, wk, num_sms, s);
+    CUtensorMap tq = {};
+    if (query_map(kv, a, &tq)) {
+        if (kv.D == 64) return launch<T, 64, true>(kv, a, tq, wk, num_sms, s);
+        if (kv.D == 128) return launch<T, 128, true>(kv, a, tq, wk, num_sms, s);
+        return launch<T, 256, true>(kv, a, tq, wk, num_sms, s);
+    }
+    if (kv.D == 64) return launch<T, 64, false>(kv, a, tq, wk, num_sms, s);
+    if (kv.D == 128) return launch<T, 128, false>(kv, a, tq, wk, num_sms, s);
+    return launch<T, 256, false>(kv, a, tq, wk, num_sms, s);
 }
 
 }  // namespace

@@ -94,6 +94,14 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+// Three-dimensional tensor copy into this CTA's shared memory, completing on `bar`.
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* tm, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
 // Four-dimensional tensor copy into this CTA's shared memory, completing on `bar`.
 __device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* tm, int x, int slot, int head, int page, uint64_t* bar) {
     asm volatile(
