@@ -6,7 +6,6 @@ loading fails loudly when it is missing -- there is no CPU fallback.
 
 import ctypes
 import os
-import struct
 import subprocess
 import threading
 
@@ -81,14 +80,6 @@ class RtQwen35Layer(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("gate", "up", "down", "input_norm", "post_attn_norm", "in_qkv", "in_z",
                                                "in_a", "in_b", "out_proj", "conv1d_weight", "a_log", "dt_bias",
                                                "norm_weight", "q", "k", "v", "o", "q_norm", "k_norm")]
-
-
-# The rt_paged_* argument structs, packed with native alignment (a packed bytes
-# object is passed where the C ABI takes a pointer to the struct).
-RT_PAGED_KV = struct.Struct("@2P4q4iPq2iP")         # rt_paged_kv
-RT_PAGED_ROWS = struct.Struct("@2P3qiP")            # rt_paged_rows
-RT_PAGED_ATTN = struct.Struct("@2P4qP2q4ifi2P2qPQ")  # rt_paged_attn
-RT_PAGED_EVICT = struct.Struct("@2P2q4iPq2P")       # rt_paged_evict_args
 
 
 _vp = ctypes.c_void_p
