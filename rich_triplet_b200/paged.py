@@ -106,3 +106,117 @@ def kv_evict(k_pages, v_pages, page_table, lens, mass, dst_table, *, budget, sin
     budget] int32, -1 after the last; new lengths [sequences] int32; the kept
     positions' mass in a tensor like ``mass``, zero after the last)."""
     return _ext.evict(k_pages, v_pages, page_table, lens, mass, dst_table, budget, sinks, recent)
+
+
+class PagePool:
+    """Page numbers 0 .. num_pages - 1, handed out and taken back on the host."""
+
+    def __init__(self, num_pages):
+        self.num_pages = int(num_pages)
+        self._free = list(range(self.num_pages - 1, -1, -1))
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def take(self, n):
+        if n > len(self._free):
+            raise ValueError(f"PagePool: {n} pages wanted, {len(self._free)} of {self.num_pages} free")
+        return [self._free.pop() for _ in range(n)]
+
+    def give(self, pages):
+        self._free.extend(pages)
+
+
+class PagedKvCache:
+    """The paged caches of several layers that keep the same positions of a set
+    of sequences: one pool of keys and one of values per layer, one page table
+    and one list of lengths for all of them.
+
+    ``totals`` keeps a running total of every cached position's attention
+    weight per layer ([layers, sequences, kv_heads, max_len] f32), which decode
+    and prompt add to and evict ranks by.  Lengths and the table live on the
+    host and are copied to the device when they change; the operators run on
+    torch's current stream."""
+
+    def __init__(self, layers, sequences, num_pages, page_size, kv_heads, head_dim, max_len, dtype=torch.bfloat16,
+                 device="cuda", totals=False):
+        shape = (layers, num_pages, kv_heads, page_size, head_dim)
+        self.k, self.v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        self.page_size, self.max_len, self.device = page_size, max_len, self.k.device
+        self.pool = PagePool(num_pages)
+        self.lens = [0] * sequences
+        width = -(-max_len // page_size)
+        self._table = torch.full((sequences, width), -1, dtype=torch.int32)
+        self.page_table = self._table.to(self.device)
+        self.lens_device = torch.zeros(sequences, dtype=torch.int32, device=self.device)
+        self.mass = None
+        if totals:
+            self.mass = torch.zeros((layers, sequences, kv_heads, max_len), dtype=torch.float32, device=self.device)
+
+    def _upload(self):
+        self.page_table.copy_(self._table)
+        self.lens_device.copy_(torch.tensor(self.lens, dtype=torch.int32))
+
+    def extend(self, counts):
+        """Room for counts[b] new tokens of every sequence b: lengths grow and
+        pages are taken from the pool."""
+        wanted = [n + c for n, c in zip(self.lens, counts)]
+        if len(counts) != len(self.lens) or max(wanted) > self.max_len:
+            raise ValueError(f"PagedKvCache.extend: lengths {wanted} for {len(self.lens)} sequences of at most "
+                             f"{self.max_len} positions")
+        need = [range(-(-n // self.page_size), -(-w // self.page_size)) for n, w in zip(self.lens, wanted)]
+        pages = self.pool.take(sum(len(r) for r in need))
+        for b, r in enumerate(need):
+            for p in r:
+                self._table[b, p] = pages.pop()
+        self.lens = wanted
+        self._upload()
+
+    def drop(self, window, sinks=0):
+        """Give back the pages that no later token sees: before the window of
+        the next one, and past the first ``sinks`` positions."""
+        first = -(-sinks // self.page_size)
+        for b, n in enumerate(self.lens):
+            for p in range(first, max(0, n + 1 - window) // self.page_size):
+                if self._table[b, p] >= 0:
+                    self.pool.give([int(self._table[b, p])])
+                    self._table[b, p] = -1
+        self._upload()
+
+    def append(self, layer, k, v, q_start=None):
+        kv_append(self.k[layer], self.v[layer], k, v, self.page_table, self.lens_device, q_start)
+
+    def decode(self, layer, q, *, scale, window=0, sinks=0):
+        mass = None if self.mass is None else self.mass[layer]
+        return attend_decode(q, self.k[layer], self.v[layer], self.page_table, self.lens_device, scale=scale,
+                             window=window, sinks=sinks, mass=mass)
+
+    def prompt(self, layer, q, q_start, max_new, *, scale, window=0, sinks=0):
+        mass = None if self.mass is None else self.mass[layer]
+        return attend_prompt(q, q_start, max_new, self.k[layer], self.v[layer], self.page_table, self.lens_device,
+                             scale=scale, window=window, sinks=sinks, mass=mass)
+
+    def evict(self, budget, sinks=0, recent=0):
+        """Trim every sequence of every layer to ``budget`` positions by its
+        totals (kv_evict); the old pages go back to the pool.  Returns the kept
+        positions of each layer."""
+        if self.mass is None:
+            raise ValueError("PagedKvCache.evict: the cache was made without totals")
+        each = -(-budget // self.page_size)
+        dst = torch.tensor(self.pool.take(each * len(self.lens)), dtype=torch.int32).view(len(self.lens), each)
+        on_device = dst.to(self.device)
+        kept = []
+        for i in range(self.k.shape[0]):
+            got, _, self.mass[i] = kv_evict(self.k[i], self.v[i], self.page_table, self.lens_device, self.mass[i],
+                                            on_device, budget=budget, sinks=sinks, recent=recent)
+            kept.append(got)
+        self.pool.give([int(p) for p in self._table.flatten() if p >= 0])
+        self.lens = [min(n, budget) for n in self.lens]
+        self._table.fill_(-1)
+        for b, n in enumerate(self.lens):
+            used = -(-n // self.page_size)
+            self._table[b, :used] = dst[b, :used]
+            self.pool.give(dst[b, used:].tolist())
+        self._upload()
+        return kept
