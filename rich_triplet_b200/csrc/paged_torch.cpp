@@ -54,6 +54,7 @@ bool done(int rc, rt_ctx* ctx) {
 }
 
 const at::Tensor* tensor(PyObject* o, const char* name) {
+    if (PyErr_Occurred()) return nullptr;  // an argument before this one was refused
     if (!THPVariable_Check(o)) {
         PyErr_Format(PyExc_ValueError, "%s must be a tensor", name);
         return nullptr;
