@@ -113,6 +113,7 @@ size_t paged_counter_bytes(int num_sms);
 size_t paged_decode_scratch(const PagedKv& kv, const PagedAttn& a);
 cudaError_t paged_decode_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, void* scratch, int num_sms,
                                 cudaStream_t s);
+cudaError_t paged_prompt32_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s);
 size_t paged_prompt_part_bytes(int num_sms);
 bool paged_pool_map(const PagedKv& kv, void* pool, CUtensorMap* out);
 cudaError_t paged_prompt_mass16_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s);

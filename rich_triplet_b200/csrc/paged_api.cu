@@ -90,6 +90,8 @@ int make_attn(rt_ctx* ctx, const char* who, const rt_paged_kv* kv, const rt_page
     if (prompt) {
         if (in->max_new < 0) return fail(ctx, RT_E_INVAL, "%s: negative max_new", who);
         if (in->rows > 0 && !in->q_start) return fail(ctx, RT_E_INVAL, "%s: null q_start", who);
+        if (kv->fmt == RT_FMT_F32 && in->rows * (in->num_heads / kv->kv_heads) > (1 << 25))
+            return fail(ctx, RT_E_SHAPE, "%s: at most 2^25 rows x query heads to a KV head over an f32 cache", who);
     } else {
         if (in->q_start) return fail(ctx, RT_E_INVAL, "%s: q_start belongs to rt_paged_prompt", who);
         if (in->rows != kv->num_seqs)
