@@ -140,12 +140,13 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
     const int b = static_cast<int>(bid % bhs) / kv.nkv, h = static_cast<int>(bid % bhs) % kv.nkv;
     const int64_t q_first = a.q_start[b];
     const int all = a.q_start[b + 1] - static_cast<int>(q_first), len = kv.len(b);
-    const int64_t R = min(static_cast<int64_t>(min(all, a.max_new)), a.rows - q_first) * G;
-    const int64_t row0 = static_cast<int64_t>(ytile) * NQ * kRows;
+    // (rows * G fits 32 bits: checked by the caller)
+    const int R = static_cast<int>(min(static_cast<int64_t>(min(all, a.max_new)), a.rows - q_first)) * G;
+    const int row0 = ytile * NQ * kRows;
     if (all <= 0 || q_first < 0 || row0 >= R) return;
-    const int nrows = static_cast<int>(min(R - row0, static_cast<int64_t>(NQ * kRows)));
+    const int nrows = min(R - row0, NQ * kRows);
     const int pos0 = len - all;  // position of the sequence's first new token (may be negative)
-    const int t_min = pos0 + static_cast<int>(row0 / G), t_max = pos0 + static_cast<int>((row0 + nrows - 1) / G);
+    const int t_min = pos0 + row0 / G, t_max = pos0 + (row0 + nrows - 1) / G;
     const Walk walk = make_walk(t_min, t_max, a.window, a.sinks);
     const int ns = max(1, min(wk.nsplit, (walk.count + 1) / 2));
     if (split >= ns) return;
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
     // key tiles of each query tile: those up to its last row's position
     auto tiles_of = [&](int t) -> int {
         if (t * kRows >= nrows) return 0;
-        const int last = pos0 + static_cast<int>((row0 + min(nrows, (t + 1) * kRows) - 1) / G);
+        const int last = pos0 + (row0 + min(nrows, (t + 1) * kRows) - 1) / G;
         if (last < 0) return 0;
         return max(0, min(n, walk.first_tiles + last / kKeys + 1 - walk.w_tile - i0));
     };
@@ -358,8 +359,8 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         {
             // Q tile t into shared memory, rows past the end zero: a warp its own 32 rows
             constexpr int CPR = D / 8, RPI = 32 / CPR;  // 16-byte chunks of a row; rows of a warp-wide load
-            const int own = r < nrows ? static_cast<int>((row0 + r) / G) : -1;  // this lane's row: its token
-            const int64_t off = own < 0 ? -1 : (q_first + own) * a.q_row + (h * G + static_cast<int>(row0 + r - static_cast<int64_t>(own) * G)) * a.q_head;
+            const int own = r < nrows ? (row0 + r) / G : -1;  // this lane's row: its token
+            const int64_t off = own < 0 ? -1 : (q_first + own) * a.q_row + (h * G + row0 + r - own * G) * a.q_head;
             const int ch = lane % CPR;
             uint8_t* dst = sm + t * C::kQTile + (ch >> 3) * C::kChunk + (warp & 3) * 32 * 128;
 #pragma unroll 1
@@ -381,12 +382,11 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
-        const int64_t rho = row0 + r;
+        const int rho = row0 + r;
         const bool live = r < nrows;
-        const int tok = live ? static_cast<int>(rho / G) : 0, head = live ? h * G + static_cast<int>(rho % G) : 0;
+        const int tok = live ? rho / G : 0, head = live ? h * G + rho - tok * G : 0;
         const int pos = live ? pos0 + tok : -1;
-        const int tile_lo = pos0 + static_cast<int>((row0 + t * kRows) / G);
-        const int tile_hi = pos0 + static_cast<int>((row0 + min(nrows, (t + 1) * kRows) - 1) / G);
+        const int tile_lo = pos0 + (row0 + t * kRows) / G, tile_hi = pos0 + (row0 + min(nrows, (t + 1) * kRows) - 1) / G;
         const bool warp_live = t * kRows + (warp & 3) * 32 < nrows;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
@@ -425,23 +425,26 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             }
             // rows of V that no row of this CTA sees: zero (once, by the first query tile that uses them)
             if ((t == 0 || j >= n0) && (j0 + kKeys - 1 > t_max || (a.window > 0 && j0 < walk.w_min))) {
-                const int q = j0 + (warp & 3) * 32 + lane;
                 // entries up to V of the tile before have landed: full's parity is unambiguous
                 if (C::NP == 2 && j > 0) {
                     ok = tc::warp_wait(pv_done(t, j - 1), p_parity(j - 1), abort);
                     if (!ok) break;
                 }
-                const bool dead = q > t_max || (a.window > 0 && q < walk.w_min && q >= a.sinks);
+                // a warp's 32 rows, four at a time: eight lanes to the 128 bytes of a row
+                const int at = (warp & 3) * 32 + (lane >> 3);
 #pragma unroll
                 for (int sp = 0; sp < SPT; ++sp) {
                     const int e = v_seq(j) + sp, s = e % NST;
                     ok = ok && tc::warp_wait(&full[s], static_cast<uint32_t>(e / NST) & 1u, abort);
                     if (!ok) break;
-                    if (dead) {
-                        uint4* row = reinterpret_cast<uint4*>(ring + s * C::kStage + (q - j0) * 128);
-                        for (int ch = 0; ch < C::SD / 64; ++ch)
+                    uint8_t* stage = ring + s * C::kStage + (lane & 7) * 16;
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) row[ch * (C::kChunk / 16) + i] = make_uint4(0, 0, 0, 0);
+                    for (int i = 0; i < 32; i += 4) {
+                        const int q = j0 + at + i;
+                        if (q <= t_max && (a.window == 0 || q >= walk.w_min || q < a.sinks)) continue;
+#pragma unroll
+                        for (int ch = 0; ch < C::SD / 64; ++ch)
+                            *reinterpret_cast<uint4*>(stage + ch * C::kChunk + (at + i) * 128) = make_uint4(0, 0, 0, 0);
                     }
                 }
                 if (!ok) break;
@@ -615,9 +618,9 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                             wgt[row * (kMaxSplit + 1) + s] = f;
                         }
                     wgt[row * (kMaxSplit + 1) + kMaxSplit] = M == -INFINITY ? 0.f : 1.f / L;
-                    const int64_t rr = row0 + row, tk = rr / G;
+                    const int rr = row0 + row, tk = rr / G;
                     if (a.lse)
-                        a.lse[(q_first + tk) * a.lse_row + h * G + static_cast<int>(rr - tk * G)] =
+                        a.lse[(q_first + tk) * a.lse_row + h * G + rr - tk * G] =
                             M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
@@ -646,7 +649,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                     for (int q = 0; q < kBatch; ++q) {
                         const int i = i0q + q * kSoft, row = i / (D / 4);
                         if (i >= quads) continue;
-                        const int rr = static_cast<int>(row0) + row, tk = rr / G;
+                        const int rr = row0 + row, tk = rr / G;
                         const float iv = wgt[row * (kMaxSplit + 1) + kMaxSplit];
                         *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (q_first + tk) * a.out_row + (h * G + rr - tk * G) * a.out_head +
                                                   (i % (D / 4)) * 4) =
