@@ -497,6 +497,9 @@ int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_rows* row
  *   out[r][h] = sum_j softmax_j(scale * q . k_j) v_j   (cache's type)
  *   lse[r][h] = log sum_j exp(scale * q . k_j)          (f32; NULL: not wanted)
  * A token that sees nothing (an empty sequence) gets out 0 and lse -inf.
+ * Rows that no token of the call sees may hold anything.  A value row that some
+ * token sees must be finite: of rt_paged_prompt's tokens, those computed in one
+ * tile with it (128 rows of token and head) multiply it by a weight of zero.
  * mass (NULL: not wanted): f32 [num_seqs][kv_heads][>= mass_cap], strides in
  * elements; mass[b][h][j] += the attention weight of position j summed over
  * the call's tokens of sequence b and the query heads of KV head h, for every
@@ -542,8 +545,8 @@ int rt_paged_prompt(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_attn* a, 
  * hold no page that a sequence of the call still uses.  Sequences of at most
  * `budget` positions are copied whole.  sinks + recent <= budget.
  * kept[b][h][i] (i < budget; contiguous) receives the kept positions in
- * order, then -1; new_lens[b] = min(lens[b], budget); mass_out (strides of
- * mass; must not overlap it; mass_cap values a row) receives the kept
+ * order, then -1; new_lens[b] = min(lens[b], budget), not in place of lens;
+ * mass_out (strides of mass; must not overlap it; mass_cap values a row) receives the kept
  * positions' mass, then zeros.  mass_cap must cover every length: positions
  * at mass_cap or beyond count as -inf. */
 typedef struct {

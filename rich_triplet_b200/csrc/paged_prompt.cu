@@ -37,6 +37,19 @@
 // Every wait on an mbarrier gives up after a second: the CTA records
 // kErrMbarTimeout, waits (bounded) for its copies and products in flight,
 // frees its tensor memory and returns.
+//
+// Measured (B200): 8192 tokens, 32 heads on 16 of 128, all visible: 610 us,
+// 900 TFLOP/s.  There a pair of 128 x 128 tiles takes 3800 clocks where its
+// products take 2050: the chain scores -> weights (2000) -> product with V ->
+// next scores of a tile is only half hidden behind the other tile's.  6185
+// tokens in windows of 1024, 16 heads on 4 of 256: 167 us; a 128 x 128 tile
+// takes 3200 clocks (products 2050), and every 128 rows read their own 128 KB
+// of K and V a tile from L2, 10 TB/s over the GPU.  5 x 8 tokens over 2050
+// positions: 22 us, nearly all of it start (5 us), two or three tiles (2.3 us
+// each) and the join (6 us).  Tried and slower: one lane polling for a warp
+// (745 against 682 us), a third to an eighth of the exponentials as a
+// polynomial on the FMA pipe (640 against 621), the ring's first copies before
+// the CTA's first barrier (252 against 244).
 #include <math.h>
 
 #include <algorithm>
@@ -216,50 +229,49 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
     auto v_seq = [&](int j) { return SPT * (C::kAlias ? 2 * j + 1 : (j + 1 < n ? 2 * j + 2 : 2 * j + 1)); };
 
     if (warp >= C::kSoftWarps) {
-    if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == C::kSoftWarps) {
-        // ---- producer ----
-        const int rows = min(1 << kv.page_log2, kKeys), boxes = kKeys / rows;
-        const int chunk = lane / boxes, box = lane % boxes;
-        int done = 0;
-        const int total = 2 * SPT * n;
-        bool ok = true;
-        for (int e = 0; e < total && ok; ++e) {
-            // entry e of the ring: tile j, K or V, columns [col0, + SD)
-            const int tile_e = e / SPT;
-            bool is_v;
-            int j;
-            if (C::kAlias) {
-                is_v = tile_e & 1;
-                j = tile_e >> 1;
-            } else {
-                is_v = tile_e >= 2 && (!(tile_e & 1) || tile_e == 2 * n - 1);
-                if (n == 1) is_v = tile_e == 1;
-                j = is_v ? (tile_e == 2 * n - 1 ? n - 1 : tile_e / 2 - 1) : (tile_e + 1) / 2;
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == C::kSoftWarps) {
+            // ---- producer ----
+            const int rows = min(1 << kv.page_log2, kKeys), boxes = kKeys / rows;
+            const int chunk = lane / boxes, box = lane % boxes;
+            int done = 0;
+            const int total = 2 * SPT * n;
+            bool ok = true;
+            for (int e = 0; e < total && ok; ++e) {
+                // entry e of the ring: tile j, K or V, columns [col0, + SD)
+                const int tile_e = e / SPT;
+                bool is_v;
+                int j;
+                if (C::kAlias) {
+                    is_v = tile_e & 1;
+                    j = tile_e >> 1;
+                } else {
+                    is_v = tile_e >= 2 && (!(tile_e & 1) || tile_e == 2 * n - 1);
+                    if (n == 1) is_v = tile_e == 1;
+                    j = is_v ? (tile_e == 2 * n - 1 ? n - 1 : tile_e / 2 - 1) : (tile_e + 1) / 2;
+                }
+                const int col0 = (e % SPT) * C::SD;
+                const int s = e % NST;
+                const int p = walk.tile(i0 + j) * kKeys + box * rows;
+                int page = -1;
+                if (chunk < C::SD / 64 && p < len) page = kv.table[b * kv.table_stride + (p >> kv.page_log2)];
+                if (static_cast<uint32_t>(page) >= static_cast<uint64_t>(kv.num_pages)) page = static_cast<int>(kv.num_pages);
+                if (lane == 0) {
+                    ok = e < NST || tc::wait_phase(&empty[s], static_cast<uint32_t>(e / NST - 1) & 1u, abort);
+                    if (ok) mbar_arrive_expect_tx(&full[s], C::kStage);
+                    else tc::give_up(abort, a.err);
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (ok && chunk < C::SD / 64)
+                    tc::tma_4d(ring + s * C::kStage + chunk * C::kChunk + box * rows * 128, is_v ? &tm_v : &tm_k, col0 + 64 * chunk,
+                           p & ((1 << kv.page_log2) - 1), h, page, &full[s]);
+                if (ok) ++done;
             }
-            const int col0 = (e % SPT) * C::SD;
-            const int s = e % NST;
-            const int p = walk.tile(i0 + j) * kKeys + box * rows;
-            int page = -1;
-            if (chunk < C::SD / 64 && p < len) page = kv.table[b * kv.table_stride + (p >> kv.page_log2)];
-            if (static_cast<uint32_t>(page) >= static_cast<uint64_t>(kv.num_pages)) page = static_cast<int>(kv.num_pages);
-            if (lane == 0) {
-                ok = e < NST || tc::wait_phase(&empty[s], static_cast<uint32_t>(e / NST - 1) & 1u, abort);
-                if (ok) mbar_arrive_expect_tx(&full[s], C::kStage);
-                else tc::give_up(abort, a.err);
-            }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-            if (ok && chunk < C::SD / 64)
-                tc::tma_4d(ring + s * C::kStage + chunk * C::kChunk + box * rows * 128, is_v ? &tm_v : &tm_k, col0 + 64 * chunk,
-                       p & ((1 << kv.page_log2) - 1), h, page, &full[s]);
-            if (ok) ++done;
-        }
-        // no copy may still be landing when the CTA exits
-        if (lane == 0)
-            for (int e = max(0, done - NST); e < done; ++e)
-                (void)mbar_wait_timed(&full[e % NST], static_cast<uint32_t>(e / NST) & 1u);
-    } else if (warp == C::kSoftWarps + 1) {
-        {
+            // no copy may still be landing when the CTA exits
+            if (lane == 0)
+                for (int e = max(0, done - NST); e < done; ++e)
+                    (void)mbar_wait_timed(&full[e % NST], static_cast<uint32_t>(e / NST) & 1u);
+        } else if (warp == C::kSoftWarps + 1) {
             // ---- MMA issuer: the warp walks, one elected lane issues ----
             constexpr uint32_t kIdS = tc::idesc_f16(BF16, kKeys, false), kIdO = tc::idesc_f16(BF16, C::SD, true);
             int nt[NQ];
@@ -348,8 +360,6 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             __syncwarp();
             (void)mbar_wait_timed(drain, 0u);
         }
-        __syncwarp();
-    }
     } else {
         // ---- one warpgroup per query tile, one thread per row ----
         if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));

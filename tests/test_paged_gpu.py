@@ -594,3 +594,65 @@ def test_prompt_more_row_tiles_than_sms():
         check_prompt([2600, 900], [2000, 900], 16, 4, 128, 64, BF16, seed=6)
     from rich_triplet_b200 import paged
     paged.context(DEV).sync()  # raises if a wait gave up
+
+
+def test_evict_mass_shorter_than_the_sequences():
+    """Positions at or beyond the mass tensor's end rank as -inf and have no mass."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([300, 90], 2, 64, 16, F16, spare=2 * 8)
+    mass = torch.rand(2, 2, 120, device=DEV)
+    dst = c.free[:16].view(2, 8).to(DEV)
+    kept, lens, out = paged.kv_evict(c.kp, c.vp, c.table, c.lens_t, mass, dst, budget=125, sinks=2, recent=3)
+    assert lens.tolist() == [125, 90]
+    # all 120 ranked positions, the last three, and two of the others: the lowest
+    assert kept[0, 0].tolist() == list(range(122)) + [297, 298, 299]
+    assert torch.equal(out[0], mass[0]) and torch.equal(out[1, :, :90], mass[1, :, :90]) and (out[1, :, 90:] == 0).all()
+
+
+def test_first_call_on_a_stream_inside_a_capture_is_refused():
+    """The stream's workspace cannot be made there; the capture stays usable."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([40], 2, 128, 16, BF16)
+    q = queries(1, 4, 128, BF16, 0, False)
+    want, _ = paged.attend_decode(q, *c.args(), scale=0.1)
+    s = torch.cuda.Stream(priority=-1)
+    x = torch.zeros(4, device=DEV)
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        with pytest.raises(RtError, match="workspace does not exist"):
+            paged.attend_decode(q, *c.args(), scale=0.1)
+        x += 1
+    g.replay()
+    torch.cuda.synchronize()
+    assert x.tolist() == [1, 1, 1, 1]
+    assert torch.equal(paged.attend_decode(q, *c.args(), scale=0.1)[0], want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_sequences_and_strided_tables(dtype):
+    """More sequences than threads of a CTA, lengths of zero among them, a page
+    table that is a slice of a wider one, outputs into a given strided tensor."""
+    from rich_triplet_b200 import paged
+
+    lens = [(7 * i) % 45 for i in range(700)]
+    c = Cache(lens, 1, 64, 8, dtype, seed=3)
+    wide = torch.full((700, c.table.shape[1] + 9), 10 ** 8, dtype=torch.int32, device=DEV)
+    wide[:, 4:4 + c.table.shape[1]] = c.table
+    table = wide[:, 4:4 + c.table.shape[1]]
+    q = queries(700, 2, 64, dtype, 0, True)
+    room = torch.full((700, 5, 64), 9.0, dtype=dtype, device=DEV)
+    out, lse = paged.attend_decode(q, c.kp, c.vp, table, c.lens_t, scale=0.125, out=room[:, 1:3])
+    assert out.data_ptr() == room[:, 1:3].data_ptr()
+    assert (room[:, 0] == 9).all() and (room[:, 3:] == 9).all()
+    for b in range(0, 700, 13):
+        o, ob, z, zb, _, _ = reference(c, b, q[b:b + 1], torch.tensor([lens[b] - 1], device=DEV), 0.125, 0, 0)
+        close(out[b:b + 1], o, ob, f"out of sequence {b}")
+        close(lse[b:b + 1], z, zb, f"lse of sequence {b}")
+    start = torch.arange(701, dtype=torch.int32, device=DEV)
+    again, _ = paged.attend_prompt(q, start, 1, c.kp, c.vp, table, c.lens_t, scale=0.125)
+    for b in range(0, 700, 13):
+        o, ob, _, _, _, _ = reference(c, b, q[b:b + 1], torch.tensor([lens[b] - 1], device=DEV), 0.125, 0, 0)
+        close(again[b:b + 1], o, ob, f"prompt out of sequence {b}")
