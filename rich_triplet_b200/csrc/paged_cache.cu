@@ -205,7 +205,9 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedKv kv
                     const int c = hist[top - i];
                     if (above < want && above + c >= want) {
                         s_prefix = last | static_cast<uint32_t>(top - i) << shift;
-                        s_want = want - above;
+                        // all of the digit's keys are kept: keys from `prefix` on, without a later pass
+                        s_want = want - above == c ? 0 : want - above;
+                        if (s_want == 0) s_prefix -= 1u;
                     }
                     above += c;
                 }
@@ -214,6 +216,7 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedKv kv
             last = s_prefix;
             want = s_want;
             __syncthreads();
+            if (want == 0) break;
         }
     }
     int done = 0, equal = 0;  // kept so far; keys equal to `last` so far
