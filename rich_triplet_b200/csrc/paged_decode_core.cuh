@@ -27,12 +27,13 @@
 // in two 16-bit parts (hi + lo) before they multiply V, so their rounding
 // (2^-16) stays below the output's; with G <= 4 the low parts ride in columns
 // 4..7 of the same product.  f32 rows: tf32 products of hi and lo parts of
-// both operands (hi hi + lo hi + hi lo), relative error about 2^-22.
+// both operands, relative error about 2^-22; for the scores the queries are the
+// 16-row operand, hi parts above lo parts, so two products give all four terms.
 //
 // Measured (B200): one sequence of 131071 positions, 8 heads on 4 of 256, bf16:
 // 95 us, 5.6 TB/s (the SMs finish between 62 and 84 us, the join of 74 parts
-// takes 8).  64 sequences, 1.05 GB of f32: 200 us,
-// 5.2 TB/s.  64 windows of 1028: 46 us, 5.8 TB/s.  301 positions: 9.2 us, six
+// takes 8).  64 sequences, 1.05 GB of f32: 190 us,
+// 5.5 TB/s.  64 windows of 1028: 46 us, 5.8 TB/s.  301 positions: 9.2 us, six
 // dependent trips to memory (length, page, rows, part, counter, parts).
 //
 // The maximum is only moved when a score exceeds it by more than 8 (powers of
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                 for (int i = 0; i < COPIES; ++i) {
                     // a warp-wide copy is 32 / CPR rows, or a part of one
                     const int r = CPR >= 32 ? i / (CPR / 32) : i * (32 / CPR) + lane / CPR, part = CPR >= 32 ? i % (CPR / 32) : 0;
-                    const int sw = F32 ? 2 * (r & 3) + (r >> 2) : (r & 7), ch = part * 32 + lane % CPR;
+                    const int sw = r & 7, ch = part * 32 + lane % CPR;
                     const uint32_t to = dst + r * C::kRowBytes + ((ch ^ sw) << 4);
                     const int64_t o = lds64(rows_at + r * 8);
                     if (whole_tile) cp16_all(to, base + o + part * 512);
@@ -410,8 +411,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                 if (col < ncol) {
                     const float* qr = static_cast<const float*>(a.q) + static_cast<int64_t>(row_at(col)) * a.q_row + head_at(col) * a.q_head +
                                       8 * k + (l & 3);
-                    split_tf32(qr[0], f.x, f.z);
-                    split_tf32(qr[4], f.y, f.w);
+                    split_tf32(qr[0], f.x, f.y);
+                    split_tf32(qr[4], f.z, f.w);
                 }
                 qs[i] = f;
             }
@@ -419,7 +420,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
         }
 
         float o[NT][MT][4];
-        float m[NT][2], l[NT][2];  // of columns 2 t4 and 2 t4 + 1; l: this lane's positions only
+        // of columns 2 t4 and 2 t4 + 1 (f32 rows: [0] of column g8); l: this lane's positions only
+        float m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -429,13 +431,13 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
             m[n][0] = m[n][1] = -INFINITY;
             l[n][0] = l[n][1] = 0.f;
         }
-        int when[NT][2];  // FEW: positions of the tokens of columns 2 t4 and 2 t4 + 1, -1 for no column
+        int when[NT][2];  // FEW: positions of the tokens of those columns, -1 for no column
         if constexpr (FEW) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    const int col = n * 8 + 2 * t4 + q;
+                    const int col = n * 8 + (F32 ? g8 : 2 * t4 + q);
                     when[n][q] = col < ncol ? tk.pos0 + (row0 + col) / G : -1;
                 }
         }
@@ -474,18 +476,18 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                     for (int e = 0; e < 4; ++e) s[n][e] = (acc[0][n][e] + acc[1][n][e]) * wk.scale2;
             } else {
                 const uint4* qs = reinterpret_cast<const uint4*>(smem + C::kOffQ) + lane;
+                // Rows 0..7 of the left operand are the columns' high parts, 8..15 their
+                // low parts, the eight positions its columns: S = [q_hi; q_lo] (k_hi + k_lo)^T.
                 const int r = lane & 7;
-                const int sw = 2 * (r & 3) + (r >> 2);
-                const uint32_t at[2] = {ks + r * C::kRowBytes + (((lane >> 3) ^ sw) << 4),
-                                        ks + r * C::kRowBytes + (((4 + (lane >> 3)) ^ sw) << 4)};
+                const uint32_t at[2] = {ks + r * C::kRowBytes + (((lane >> 3) ^ r) << 4),
+                                        ks + r * C::kRowBytes + (((4 + (lane >> 3)) ^ r) << 4)};
                 // The tensor cores' f32 sums cut off instead of rounding: four short
                 // chains for the large products, added here.
-                float hh[4][NT][4], lh[NT][4], hl[NT][4];
+                float hh[4][NT][4], lo[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        hh[0][n][e] = hh[1][n][e] = hh[2][n][e] = hh[3][n][e] = lh[n][e] = hl[n][e] = 0.f;
+                    for (int e = 0; e < 4; ++e) hh[0][n][e] = hh[1][n][e] = hh[2][n][e] = hh[3][n][e] = lo[n][e] = 0.f;
 #pragma unroll 4
                 for (int k2 = 0; k2 < D / 16; ++k2) {  // chain 2 (k2 % 2) + k of hh
                     uint32_t kf[4];
@@ -498,65 +500,76 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             const uint4 f = qs[(n * (D / 8) + 2 * k2 + k) * 32];
-                            mma8(hh[2 * (k2 & 1) + k][n], h0, 0u, h1, 0u, f.x, f.y);
-                            mma8(lh[n], l0, 0u, l1, 0u, f.x, f.y);
-                            mma8(hl[n], h0, 0u, h1, 0u, f.z, f.w);
+                            mma8(hh[2 * (k2 & 1) + k][n], f.x, f.y, f.z, f.w, h0, h1);
+                            mma8(lo[n], f.x, f.y, f.z, f.w, l0, l1);
                         }
                     }
                 }
+                // column g8, positions 2 t4 and 2 t4 + 1
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[n][e] = ((hh[0][n][e] + hh[1][n][e]) + (hh[2][n][e] + hh[3][n][e]) + (lh[n][e] + hl[n][e])) * wk.scale2;
+                    for (int e = 0; e < 2; ++e)
+                        s[n][e] = ((hh[0][n][e] + hh[1][n][e]) + (hh[2][n][e] + hh[3][n][e]) +
+                                   (((hh[0][n][e + 2] + hh[1][n][e + 2]) + (hh[2][n][e + 2] + hh[3][n][e + 2])) +
+                                    (lo[n][e] + lo[n][e + 2]))) * wk.scale2;
+                    s[n][2] = s[n][3] = -INFINITY;
+                }
             }
             slot = slot + 1 == NS ? 0 : slot + 1;
             // ---- weights ----
-            constexpr int EL = F32 ? 2 : 4;  // values of a lane: rows g8 and, 16-bit tiles, g8 + 8
+            constexpr int EL = F32 ? 2 : 4;  // values of a lane: positions g8, g8 + 8 of two columns (f32: 2 t4, 2 t4 + 1 of one)
             bool over = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < EL; ++e) {
-                    const int c = c0 + g8 + (e >> 1) * 8;
+                    const int c = F32 ? c0 + 2 * t4 + e : c0 + g8 + (e >> 1) * 8, q = F32 ? 0 : (e & 1);
                     if (!FEW && wk.scores && c < c_end) {
-                        const int col = n * 8 + 2 * t4 + (e & 1), head = head_of<DUP>(col);
+                        const int col = n * 8 + (F32 ? g8 : 2 * t4 + q), head = head_of<DUP>(col);
                         if (head < G && (!DUP || col < 4))
                             wk.scores[(static_cast<int64_t>(b) * a.nq + h * G + head) * wk.score_stride + c] = s[n][e];
                     }
                     bool seen = c < c_end;
                     if constexpr (FEW) {
-                        const int p = vis.pos(c), t = when[n][e & 1];
+                        const int p = vis.pos(c), t = when[n][q];
                         seen = seen && p <= t && (a.window == 0 || p > t - a.window || p < a.sinks);
                     }
                     s[n][e] = seen ? s[n][e] : -INFINITY;
-                    over |= s[n][e] > m[n][e & 1] + kMaxSlack;
+                    over |= s[n][e] > m[n][q] + kMaxSlack;
                 }
             if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
+                    float f[2];
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        float v = s[n][q];
-                        if (EL == 4) v = fmaxf(v, s[n][q + 2]);
+                    for (int q = 0; q < (F32 ? 1 : 2); ++q) {
+                        float v = F32 ? fmaxf(s[n][0], s[n][1]) : fmaxf(s[n][q], s[n][q + 2]);
 #pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                        const float mn = fmaxf(m[n][q], v), f = rel2(m[n][q], mn);
+                        for (int d = F32 ? 1 : 4; d < (F32 ? 4 : 32); d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+                        const float mn = fmaxf(m[n][q], v);
+                        f[q] = rel2(m[n][q], mn);
                         m[n][q] = mn;
-                        l[n][q] *= f;
-#pragma unroll
-                        for (int j = 0; j < MT; ++j) {
-                            o[n][j][q] *= f;
-                            o[n][j][q + 2] *= f;
-                        }
+                        l[n][q] *= f[q];
                     }
+                    if (F32) {  // the output's columns are 2 t4 and 2 t4 + 1
+                        const float own = f[0];
+                        f[0] = __shfl_sync(0xffffffffu, own, 8 * t4);
+                        f[1] = __shfl_sync(0xffffffffu, own, 8 * t4 + 4);
+                    }
+#pragma unroll
+                    for (int j = 0; j < MT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[n][j][e] *= f[e & 1];
+                }
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < EL; ++e) {
-                    s[n][e] = rel2(s[n][e], m[n][e & 1]);
-                    l[n][e & 1] += s[n][e];
+                    const int q = F32 ? 0 : (e & 1);
+                    s[n][e] = rel2(s[n][e], m[n][q]);
+                    l[n][q] += s[n][e];
                 }
             // ---- O^T += V^T P^T ----
             issue();
@@ -597,20 +610,17 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {  // positions t4 and t4 + 4, column g8
-                        const int src = (t4 + 4 * q) * 4 + (g8 >> 1);
-                        const float p0 = __shfl_sync(0xffffffffu, s[n][0], src), p1 = __shfl_sync(0xffffffffu, s[n][1], src);
-                        split_tf32((g8 & 1) ? p1 : p0, ph[n][q], pl[n][q]);
-                    }
-                // value q of 16-dim tile j: dims 16 j + g8 + 8 (q & 1), positions t4 + 4 (q >> 1);
+                    for (int q = 0; q < 2; ++q) split_tf32(s[n][q], ph[n][q], pl[n][q]);  // positions 2 t4 + q, column g8
+                // value q of 16-dim tile j: dims 16 j + g8 + 8 (q & 1), positions 2 t4 + (q >> 1)
+                // (the product's steps t4 and t4 + 4 may be any two positions);
                 // its chunk 4 j + 2 (q & 1) + g8 / 4 is turned in bits 0..2 by the swizzle
                 uint32_t at[2][4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int r = t4 + 4 * (q >> 1), sw = 2 * (r & 3) + (r >> 2);
+                    const int r = 2 * t4 + (q >> 1);
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
-                        at[j][q] = vs + r * C::kRowBytes + (((4 * j + 2 * (q & 1) + (g8 >> 2)) ^ sw) << 4) + (g8 & 3) * 4;
+                        at[j][q] = vs + r * C::kRowBytes + (((4 * j + 2 * (q & 1) + (g8 >> 2)) ^ r) << 4) + (g8 & 3) * 4;
                 }
 #pragma unroll
                 for (int j = 0; j < MT; ++j) {
@@ -639,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) l[n][q] += __shfl_xor_sync(0xffffffffu, l[n][q], d);
+                for (int d = F32 ? 1 : 4; d < (F32 ? 4 : 32); d <<= 1) l[n][q] += __shfl_xor_sync(0xffffffffu, l[n][q], d);
         __syncthreads();  // every warp is done with its ring (and the query fragments)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -651,7 +661,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                     row[16 * j + g8] = o[n][j][q];
                     row[16 * j + g8 + 8] = o[n][j][q + 2];
                 }
-                if (g8 == 0) ml[warp * NT * 8 + n * 8 + 2 * t4 + q] = make_float2(m[n][q], l[n][q]);
+                if (!F32 && g8 == 0) ml[warp * NT * 8 + n * 8 + 2 * t4 + q] = make_float2(m[n][q], l[n][q]);
+                if (F32 && q == 0 && t4 == 0) ml[warp * NT * 8 + n * 8 + g8] = make_float2(m[n][0], l[n][0]);
             }
         }
         __syncthreads();
