@@ -61,11 +61,11 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedKv kv, con
     for (int i = threadIdx.x; i < kv.nkv * per; i += blockDim.x) {
         const int h = i / per, d = (i % per) * 8;
         const int64_t src = r * a.row_stride + h * a.head_stride + d, dst = off + h * kv.head_stride + d;
-        float x[8];
+        float x[8], y[8];
         load8(static_cast<const S*>(a.k) + src, x);
+        load8(static_cast<const S*>(a.v) + src, y);
         store8(static_cast<T*>(kv.k) + dst, x);
-        load8(static_cast<const S*>(a.v) + src, x);
-        store8(static_cast<T*>(kv.v) + dst, x);
+        store8(static_cast<T*>(kv.v) + dst, y);
     }
 }
 
