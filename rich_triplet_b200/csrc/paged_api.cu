@@ -197,13 +197,16 @@ int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* in, const rt_paged_rows* r, 
 
 int rt_paged_scratch(const rt_paged_kv* in, const rt_paged_attn* at, int32_t prompt, uint64_t* bytes) {
     if (!in || !at || !bytes) return RT_E_INVAL;
-    if (in->page_size < 1 || at->rows < 0 || in->table_width < 0 || at->num_heads < 1) return RT_E_SHAPE;
+    if (in->page_size < 1 || at->rows < 0 || in->table_width < 0 || at->num_heads < 1 || at->window < 0 || at->sinks < 0)
+        return RT_E_SHAPE;
     rt::PagedKv kv = {};
     rt::PagedAttn a = {};
     kv.width = in->table_width;
     while ((1 << kv.page_log2) < in->page_size) ++kv.page_log2;
     a.rows = at->rows;
     a.nq = at->num_heads;
+    a.window = at->window;
+    a.sinks = at->sinks;
     a.mass = at->mass;
     a.lse = at->lse;
     *bytes = scratch_need(kv, a, prompt != 0);

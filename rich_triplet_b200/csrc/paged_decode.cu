@@ -50,10 +50,16 @@ size_t paged_workspace_bytes(int num_sms) {
 
 size_t paged_counter_bytes(int num_sms) { return (decode_grid(num_sms) * sizeof(uint32_t) + 255) / 256 * 256; }
 
+// Scores of a (sequence, head): at most the positions that a token can see.
+static int64_t score_stride(const PagedKv& kv, const PagedAttn& a) {
+    const int64_t cap = static_cast<int64_t>(kv.width) << kv.page_log2;
+    return a.window > 0 ? std::min<int64_t>(cap, static_cast<int64_t>(a.window) + a.sinks) : cap;
+}
+
 size_t paged_decode_scratch(const PagedKv& kv, const PagedAttn& a) {
     if (!a.mass) return 0;
-    const size_t rows = static_cast<size_t>(a.rows) * a.nq, cap = static_cast<size_t>(kv.width) << kv.page_log2;
-    return (rows * sizeof(float2) + 255) / 256 * 256 + (rows * cap * sizeof(float) + 255) / 256 * 256;
+    const size_t rows = static_cast<size_t>(a.rows) * a.nq;
+    return (rows * sizeof(float2) + 255) / 256 * 256 + (rows * score_stride(kv, a) * sizeof(float) + 255) / 256 * 256;
 }
 
 cudaError_t paged_decode_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, void* scratch, int num_sms,
@@ -66,15 +72,14 @@ cudaError_t paged_decode_launch(const PagedKv& kv, const PagedAttn& a, void* wor
         const size_t rows = static_cast<size_t>(a.rows) * a.nq;
         wk.norm = static_cast<float2*>(scratch);
         wk.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + (rows * sizeof(float2) + 255) / 256 * 256);
-        wk.score_stride = static_cast<int64_t>(kv.width) << kv.page_log2;
+        wk.score_stride = score_stride(kv, a);
     }
     const int grid = decode_grid(num_sms);
     const cudaError_t e = kv.type == kPagedF32 ? by_dim<float>(kv, a, wk, grid, s)
                         : kv.type == kPagedF16 ? by_dim<__half>(kv, a, wk, grid, s)
                                                : by_dim<__nv_bfloat16>(kv, a, wk, grid, s);
     if (e != cudaSuccess || !a.mass) return e;
-    int64_t n = wk.score_stride;
-    if (a.window > 0) n = std::min<int64_t>(n, static_cast<int64_t>(a.window) + a.sinks);
+    const int64_t n = wk.score_stride;
     if (n == 0) return cudaSuccess;
     return rt_launch(paged_decode_mass_kernel, dim3(static_cast<unsigned>((n + 255) / 256), kv.nkv, kv.nseq), 256, 0, s, true, kv, a, wk);
 }
