@@ -361,11 +361,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
         int64_t off_next = row_of(0);
         auto issue = [&]() {
             const int half = issued & 1;
+            __syncwarp();  // every lane has read the last tile's offsets, and the slot that is filled here
             if (half == 0) {
-                __syncwarp();  // the last tile's offsets have been read
                 if (lane < ROWS) sts64(rows_at + lane * 8, off_next < 0 ? -1 : off_next * static_cast<int64_t>(sizeof(T)));
                 whole_tile = __all_sync(0xffffffffu, off_next >= 0);
                 off_next = row_of((issued >> 1) + 1);
+                __syncwarp();  // the offsets are there for the other lanes (a vote orders no memory)
             }
             if (issued < 2 * tiles) {
                 const char* base = half ? vl : kl;
