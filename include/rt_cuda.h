@@ -465,8 +465,8 @@ typedef struct {
     int64_t page_stride, head_stride, slot_stride; /* elements */
     int64_t num_pages;
     int32_t fmt, kv_heads, head_dim, page_size;
-    const int32_t* page_table;                     /* [num_seqs][table_stride] */
-    int64_t table_stride;
+    const int32_t* page_table;
+    int64_t table_stride;                          /* entries from one sequence's row to the next; 0: one row for all */
     int32_t table_width;                           /* entries of a row that may be read */
     int32_t num_seqs;
     const int32_t* lens;                           /* [num_seqs] */

@@ -53,7 +53,7 @@ int make_kv(rt_ctx* ctx, const char* who, const rt_paged_kv* in, rt::PagedKv* ou
         return fail(ctx, RT_E_SHAPE, "%s: num_pages %lld out of range", who, static_cast<long long>(in->num_pages));
     if (in->num_seqs < 0 || in->num_seqs > 65535)
         return fail(ctx, RT_E_SHAPE, "%s: num_seqs %d out of range (0..65535)", who, in->num_seqs);
-    if (in->table_width < 0 || in->table_stride < in->table_width ||
+    if (in->table_width < 0 || in->table_stride < 0 ||
         static_cast<int64_t>(in->table_width) * in->page_size > INT32_MAX - 256 ||
         static_cast<int64_t>(in->table_width) * in->page_size * in->num_seqs > (int64_t{1} << 44))
         return fail(ctx, RT_E_SHAPE, "%s: page table of width %d, row stride %lld", who, in->table_width,

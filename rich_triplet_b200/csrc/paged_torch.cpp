@@ -121,7 +121,7 @@ bool get_cache(PyObject* const* a, Cache* c) {
     kv.head_dim = static_cast<int32_t>(k->size(3));
     kv.page_size = static_cast<int32_t>(k->size(2));
     kv.page_table = static_cast<const int32_t*>(table->data_ptr());
-    kv.table_stride = std::max(table->stride(0), width);
+    kv.table_stride = n > 1 ? table->stride(0) : width;  // the stride of an extent of one is arbitrary
     kv.table_width = static_cast<int32_t>(width);
     kv.num_seqs = static_cast<int32_t>(n);
     kv.lens = static_cast<const int32_t*>(lens->data_ptr());

@@ -32,3 +32,33 @@ def test_decode_does_not_depend_on_where_pages_lie(dtype, nq, nkv, d):
         table = torch.where(c.table >= 0, to[c.table.clamp(min=0).long()].int(), c.table)
         got = paged.attend_decode(q, kp, vp, table, c.lens_t, scale=d ** -0.5)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_table_row_for_all_sequences(dtype):
+    """Samples that share one prompt's pages: an expanded table (row stride 0),
+    and a view whose rows overlap, give what a copy of the rows gives."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([500], 2, 64, 16, dtype, spare=12)
+    lens = torch.tensor([500, 17, 0, 333], dtype=torch.int32, device=DEV)
+    shared = c.table.expand(4, -1)
+    sliding = torch.as_strided(c.table, (4, 20), (3, 1))  # sequence b starts three pages after b - 1
+    assert shared.stride(0) == 0 and sliding.stride(0) < sliding.size(1)
+    for table, n in ((shared, lens), (sliding, lens.clamp(max=320))):
+        copied = table.clone(memory_format=torch.contiguous_format)
+        q = queries(4, 4, 64, dtype, 1, False)
+        mass = [torch.zeros(4, 2, 512, device=DEV) for _ in range(4)]
+        got = paged.attend_decode(q, c.kp, c.vp, table, n, scale=0.125, mass=mass[0])
+        want = paged.attend_decode(q, c.kp, c.vp, copied, n, scale=0.125, mass=mass[1])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(mass[0], mass[1])
+        start = torch.tensor([0, 5, 9, 9, 20], dtype=torch.int32, device=DEV)
+        q = queries(20, 4, 64, dtype, 2, False)
+        got = paged.attend_prompt(q, start, 11, c.kp, c.vp, table, n, scale=0.125, mass=mass[2])
+        want = paged.attend_prompt(q, start, 11, c.kp, c.vp, copied, n, scale=0.125, mass=mass[3])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(mass[2], mass[3])
+        dst = c.free[:12].view(4, 3).to(DEV)
+        total = torch.rand(4, 2, 512, device=DEV)
+        kept = paged.kv_evict(c.kp, c.vp, table, n, total, dst, budget=40)
+        again = paged.kv_evict(c.kp, c.vp, copied, n, total, dst, budget=40)
+        assert all(torch.equal(x, y) for x, y in zip(kept, again))
