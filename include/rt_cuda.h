@@ -504,7 +504,9 @@ int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_rows* row
  * elements; mass[b][h][j] += the attention weight of position j summed over
  * the call's tokens of sequence b and the query heads of KV head h, for every
  * visible j < mass_cap: the running total that rt_paged_evict ranks by.
- * Results do not depend on launch order: every sum has a fixed order.
+ * Results do not depend on launch order: every sum has a fixed order.  Rows of
+ * out, and rows of mass, that overlap one another (a stride of 0, say) are
+ * refused.
  *
  * rt_paged_decode: one token per sequence, at its last position; q_start must
  * be NULL and rows == num_seqs.  rt_paged_prompt: rows q_start[b] ..

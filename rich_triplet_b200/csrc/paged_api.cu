@@ -40,6 +40,18 @@ bool strides_ok(int esize, S... s) {
     return ((s >= 0 && s * esize % 16 == 0) && ...);
 }
 
+// Whether n x m rows of `len` elements, at i * si + j * sj, lie apart: rows of
+// one index hold those of the other between them.
+bool apart(int64_t n, int64_t si, int64_t m, int64_t sj, int64_t len) {
+    // the first stride spans all the rows of the second index (divided, so that nothing overflows)
+    auto nested = [len](int64_t outer, int64_t so, int64_t inner, int64_t sn) {
+        if (inner > 1 && sn < len) return false;
+        if (outer <= 1) return true;
+        return so >= len && (inner <= 1 || (so - len) / sn >= inner - 1);
+    };
+    return n <= 0 || m <= 0 || len <= 0 || nested(n, si, m, sj) || nested(m, sj, n, si);
+}
+
 int make_kv(rt_ctx* ctx, const char* who, const rt_paged_kv* in, rt::PagedKv* out) {
     const int type = paged_type(in->fmt);
     if (type < 0) return fail(ctx, RT_E_FORMAT, "%s: cache format %d is not f32, f16 or bf16", who, in->fmt);
@@ -101,9 +113,13 @@ int make_attn(rt_ctx* ctx, const char* who, const rt_paged_kv* kv, const rt_page
     if (!aligned(in->q) || !aligned(in->out) ||
         !strides_ok(esize, in->q_row_stride, in->q_head_stride, in->out_row_stride, in->out_head_stride))
         return fail(ctx, RT_E_INVAL, "%s: q and out must be 16-byte aligned with strides in multiples of 16 bytes", who);
+    if (!apart(in->rows, in->out_row_stride, in->num_heads, in->out_head_stride, kv->head_dim))
+        return fail(ctx, RT_E_SHAPE, "%s: the rows of out overlap", who);
     if (in->lse && in->lse_row_stride < in->num_heads) return fail(ctx, RT_E_SHAPE, "%s: lse rows overlap", who);
     if (in->mass && (in->mass_cap < 0 || in->mass_seq_stride < 0 || in->mass_head_stride < 0))
         return fail(ctx, RT_E_SHAPE, "%s: negative mass size or stride", who);
+    if (in->mass && !apart(kv->num_seqs, in->mass_seq_stride, kv->kv_heads, in->mass_head_stride, in->mass_cap))
+        return fail(ctx, RT_E_SHAPE, "%s: the rows of mass overlap", who);
     *out = rt::PagedAttn{in->q, in->out, in->q_row_stride, in->q_head_stride, in->out_row_stride, in->out_head_stride,
                          in->lse, in->lse_row_stride, in->rows, in->num_heads, in->num_heads / kv->kv_heads,
                          in->window, in->sinks, in->max_new, in->scale, in->mass_cap, prompt ? in->q_start : nullptr,
@@ -230,6 +246,8 @@ int rt_paged_evict(rt_ctx* ctx, const rt_paged_kv* in, const rt_paged_evict_args
         return fail(ctx, RT_E_INVAL, "%s: sinks %d + recent %d must lie in 0..budget %d", who, e->sinks, e->recent, e->budget);
     if (e->mass_cap < 0 || e->mass_seq_stride < 0 || e->mass_head_stride < 0)
         return fail(ctx, RT_E_SHAPE, "%s: negative mass size or stride", who);
+    if (!apart(in->num_seqs, e->mass_seq_stride, in->kv_heads, e->mass_head_stride, e->mass_cap))
+        return fail(ctx, RT_E_SHAPE, "%s: the rows of mass overlap", who);
     if (e->dst_stride < (static_cast<int64_t>(e->budget) + in->page_size - 1) / in->page_size)
         return fail(ctx, RT_E_SHAPE, "%s: %lld destination pages a row hold fewer than %d positions", who,
                     static_cast<long long>(e->dst_stride), e->budget);

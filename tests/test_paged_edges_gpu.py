@@ -9,6 +9,7 @@ definition are used here, except where a test says otherwise.
 import pytest
 import torch
 
+from rich_triplet_b200._lib import RtError
 from test_paged_gpu import BF16, DEV, F16, F32, Cache, queries
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +63,41 @@ def test_one_table_row_for_all_sequences(dtype):
         kept = paged.kv_evict(c.kp, c.vp, table, n, total, dst, budget=40)
         again = paged.kv_evict(c.kp, c.vp, copied, n, total, dst, budget=40)
         assert all(torch.equal(x, y) for x, y in zip(kept, again))
+
+
+def refused(error, match, fn, *args, **kw):
+    with pytest.raises(error, match=match):
+        fn(*args, **kw)
+
+
+def test_outputs_whose_rows_overlap_are_refused():
+    """Expanded totals and outputs would be written by several CTAs at once."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([40, 9], 2, 64, 16, BF16)
+    q = queries(2, 4, 64, BF16, 0, False)
+    start = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    one = torch.zeros(1, 1, 50, device=DEV)
+    wide = torch.zeros(400, device=DEV)
+    for mass in (one.expand(2, 2, -1), one.expand(2, 1, -1).repeat(1, 2, 1)[:1].expand(2, -1, -1),
+                 torch.as_strided(wide, (2, 2, 50), (49, 100, 1)), torch.as_strided(wide, (2, 2, 50), (60, 49, 1))):
+        refused(RtError, "rows of mass overlap", paged.attend_decode, q, *c.args(), scale=0.1, mass=mass)
+        refused(RtError, "rows of mass overlap", paged.attend_prompt, q, start, 1, *c.args(), scale=0.1, mass=mass)
+    for out in (torch.zeros(1, 4, 64, dtype=BF16, device=DEV).expand(2, -1, -1),
+                torch.zeros(2, 1, 64, dtype=BF16, device=DEV).expand(-1, 4, -1)):
+        refused(RtError, "rows of out overlap", paged.attend_decode, q, *c.args(), scale=0.1, out=out)
+        refused(RtError, "rows of out overlap", paged.attend_prompt, q, start, 1, *c.args(), scale=0.1, out=out)
+    # rows that lie apart in any order are taken
+    want = torch.zeros(2, 2, 50, device=DEV)
+    o, z = paged.attend_decode(q, *c.args(), scale=0.1, mass=want)
+    for mass in (torch.zeros(2, 2, 50, device=DEV).transpose(0, 1), torch.as_strided(wide, (2, 2, 50), (51, 150, 1)),
+                 torch.zeros(5, 3, 70, device=DEV)[1:4:2, 1:, 8:58]):
+        paged.attend_decode(q, *c.args(), scale=0.1, mass=mass)
+        assert torch.equal(mass, want)
+    out = torch.zeros(4, 2, 64, dtype=BF16, device=DEV).transpose(0, 1)
+    assert torch.equal(paged.attend_decode(q, *c.args(), scale=0.1, out=out)[0], o) and torch.equal(out, o)
+    # one sequence: its stride says nothing
+    c = Cache([40], 1, 64, 16, BF16)
+    mass = torch.as_strided(wide, (1, 1, 50), (0, 0, 1)).zero_()
+    paged.attend_decode(q[:1], *c.args(), scale=0.1, mass=mass)
+    assert abs(float(mass.sum()) - 4) < 1e-3
