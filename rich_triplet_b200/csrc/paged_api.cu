@@ -135,7 +135,10 @@ uint64_t scratch_need(const rt::PagedKv& kv, const rt::PagedAttn& a, bool prompt
 
 // The stream's workspace, made on first use.
 int workspace(rt_ctx* ctx, const char* who, cudaStream_t s, void** out) {
-    auto it = ctx->paged_ws.find(s);
+    // the per-thread default stream is another stream in each thread
+    static thread_local char t_own;
+    const void* key = s == cudaStreamPerThread ? static_cast<const void*>(&t_own) : static_cast<const void*>(s);
+    auto it = ctx->paged_ws.find(key);
     if (it != ctx->paged_ws.end()) {
         *out = it->second;
         return RT_OK;
@@ -151,7 +154,7 @@ int workspace(rt_ctx* ctx, const char* who, cudaStream_t s, void** out) {
         cudaFree(p);
         return fail(ctx, RT_E_CUDA, "%s: %s", who, cudaGetErrorString(e));
     }
-    ctx->paged_ws[s] = p;
+    ctx->paged_ws[key] = p;
     *out = p;
     return RT_OK;
 }

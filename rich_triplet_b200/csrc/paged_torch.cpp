@@ -19,9 +19,12 @@
 
 namespace {
 
-PyObject* g_make_context = nullptr;  // device index -> address of this thread's rt_ctx
-PyObject* g_raise = nullptr;         // (status, address of the rt_ctx): raises
-thread_local rt_ctx* t_ctx[64] = {};
+PyObject* g_make_context = nullptr;  // device index -> address of the process's rt_ctx there
+PyObject* g_raise = nullptr;         // (status, message): raises
+// The contexts that g_make_context gave, until forget(): every use of them, and
+// of this array, is made with the interpreter's lock held.
+constexpr int kDevices = 64;
+rt_ctx* g_ctx[kDevices] = {};
 
 bool value_error(const char* fmt, ...) {
     va_list ap;
@@ -32,7 +35,7 @@ bool value_error(const char* fmt, ...) {
 }
 
 rt_ctx* context(int index) {
-    if (index >= 0 && index < 64 && t_ctx[index]) return t_ctx[index];
+    if (index >= 0 && index < kDevices && g_ctx[index]) return g_ctx[index];
     PyObject* h = g_make_context ? PyObject_CallFunction(g_make_context, "i", index) : nullptr;
     if (!h) {
         if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "_paged_torch is not bound");
@@ -40,14 +43,15 @@ rt_ctx* context(int index) {
     }
     rt_ctx* ctx = static_cast<rt_ctx*>(PyLong_AsVoidPtr(h));
     Py_DECREF(h);
-    if (index < 64 && !PyErr_Occurred()) t_ctx[index] = ctx;
-    return PyErr_Occurred() ? nullptr : ctx;
+    if (PyErr_Occurred()) return nullptr;
+    if (index >= 0 && index < kDevices) g_ctx[index] = ctx;
+    return ctx;
 }
 
 // True if `rc` is RT_OK; else the error is raised.
 bool done(int rc, rt_ctx* ctx) {
     if (rc == RT_OK) return true;
-    PyObject* r = PyObject_CallFunction(g_raise, "iN", rc, PyLong_FromVoidPtr(ctx));
+    PyObject* r = g_raise ? PyObject_CallFunction(g_raise, "is", rc, ctx ? rt_last_error(ctx) : "") : nullptr;
     Py_XDECREF(r);
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "rt_paged call failed");
     return false;
@@ -310,6 +314,33 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
 }
 
+bool get_index(PyObject* const* a, Py_ssize_t n, int* out) {
+    if (n != 1) {
+        PyErr_SetString(PyExc_TypeError, "one device index is wanted");
+        return false;
+    }
+    const long v = PyLong_AsLong(a[0]);
+    *out = static_cast<int>(v);
+    return !(v == -1 && PyErr_Occurred());
+}
+
+// sync(index): rt_sync of the device's context, if there is one
+PyObject* sync(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    int index;
+    if (!get_index(a, n, &index)) return nullptr;
+    rt_ctx* ctx = index >= 0 && index < kDevices ? g_ctx[index] : nullptr;
+    if (ctx && !done(rt_sync(ctx), ctx)) return nullptr;
+    Py_RETURN_NONE;
+}
+
+// forget(index): the next call on the device asks for its context again
+PyObject* forget(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    int index;
+    if (!get_index(a, n, &index)) return nullptr;
+    if (index >= 0 && index < kDevices) g_ctx[index] = nullptr;
+    Py_RETURN_NONE;
+}
+
 // bind(make_context, raise_error)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 2) return PyErr_Format(PyExc_TypeError, "bind takes 2 arguments");
@@ -324,6 +355,8 @@ PyMethodDef g_methods[] = {
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(append)), METH_FASTCALL, "rt_paged_append"},
     {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attend)), METH_FASTCALL, "rt_paged_decode, rt_paged_prompt"},
     {"evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(evict)), METH_FASTCALL, "rt_paged_evict"},
+    {"sync", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(sync)), METH_FASTCALL, "rt_sync"},
+    {"forget", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(forget)), METH_FASTCALL, "drop a device's context"},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind)), METH_FASTCALL, "set the context factory and the error raiser"},
     {nullptr, nullptr, 0, nullptr}};
 

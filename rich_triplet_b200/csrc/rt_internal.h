@@ -32,8 +32,8 @@ struct rt_ctx {
     // intermediates).
     float* io = nullptr;
     size_t io_floats = 0;
-    // Workspace of the paged-cache calls made on each stream.
-    std::map<cudaStream_t, void*> paged_ws;
+    // Workspace of the paged-cache calls made on each stream (by its handle).
+    std::map<const void*, void*> paged_ws;
 };
 
 struct rt_w {

@@ -2,8 +2,8 @@
 
 The operators take torch tensors on the GPU and only enqueue work, on the
 current CUDA stream of the tensors' device, like torch's own operators; the
-context behind them (one per thread and device, as ops.default_context) keeps
-one workspace per stream.  They run the rt_paged_* entry points of
+context behind them, one per device for all threads of the process, keeps one
+workspace per stream.  They run the rt_paged_* entry points of
 include/rt_cuda.h, whose comments define them; the reference has one
 contiguous cache per layer instead (Gemma3LayerKvCache,
 src/transformer4.rs:1794-1864).
@@ -30,7 +30,7 @@ import threading
 
 import torch
 
-from ._lib import check, lib
+from ._lib import RT_E_STATE, RtError, lib
 from .ops import Context
 
 lib()  # raises if the library has not been built
@@ -41,31 +41,58 @@ except ImportError as e:
                        f"({e})") from e
 
 
-class _Contexts(threading.local):
-    """This thread's library contexts, by device."""
+class _DeviceContext(Context):
+    """The library context of all paged calls on one device, made on first use
+    and kept for the life of the process: the workspaces that captured graphs use
+    belong to it, whichever thread captured them.  Calls, and sync(), use it with
+    the interpreter's lock held, so threads may share it."""
 
-    def __init__(self):
-        self.made = {}
+    def sync(self):
+        """Waits for all streams of the device and raises RtError if a kernel
+        reported that a bounded wait gave up since the last sync()."""
+        torch.cuda.synchronize(self.device)
+        _ext.sync(self.device)
 
-    def get(self, index):
-        ctx = self.made.get(index)
+    def close(self):
+        """Frees the context and the workspaces of its streams: no captured graph
+        may run afterwards.  The next call makes a new one."""
+        if self.h:
+            if _made.get(self.device) is self:
+                del _made[self.device]
+                _ext.forget(self.device)
+            torch.cuda.synchronize(self.device)
+            super().close()
+
+
+_made = {}
+_making = threading.Lock()
+
+
+def _context(index):
+    with _making:
+        ctx = _made.get(index)
         if ctx is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RtError(RT_E_STATE, "the paged operators' context does not exist yet; make one call before the capture")
             before = torch.cuda.current_device()
-            ctx = self.made[index] = Context(index)
+            ctx = _DeviceContext(index)
             torch.cuda.set_device(before)
+            _made[index] = ctx
         return ctx
 
 
-_contexts = _Contexts()
-_ext.bind(lambda index: _contexts.get(index).h.value, check)
+def _raise(rc, message):
+    raise RtError(rc, message)
+
+
+_ext.bind(lambda index: _context(index).h.value, _raise)
 
 
 def context(device):
-    """This thread's library context on a GPU: its sync() waits for the
-    context's own stream and raises RtError if a kernel of any stream reported
-    that a bounded wait gave up."""
+    """The library context behind the calls on a GPU: its sync() waits for the
+    device and raises RtError if a kernel reported that a bounded wait gave up."""
     device = torch.device(device)
-    return _contexts.get(device.index if device.index is not None else torch.cuda.current_device())
+    return _context(device.index if device.index is not None else torch.cuda.current_device())
 
 
 def kv_append(k_pages, v_pages, k, v, page_table, lens, q_start=None):

@@ -6,6 +6,8 @@ Tolerances are those derived in test_paged_gpu.py, whose caches and 64-bit
 definition are used here, except where a test says otherwise.
 """
 
+import threading
+
 import pytest
 import torch
 
@@ -101,3 +103,92 @@ def test_outputs_whose_rows_overlap_are_refused():
     mass = torch.as_strided(wide, (1, 1, 50), (0, 0, 1)).zero_()
     paged.attend_decode(q[:1], *c.args(), scale=0.1, mass=mass)
     assert abs(float(mass.sum()) - 4) < 1e-3
+
+
+def test_a_closed_context_is_not_used_again():
+    from rich_triplet_b200 import paged
+
+    c = Cache([300, 41], 2, 128, 16, BF16)
+    q = queries(2, 4, 128, BF16, 0, False)
+    want = paged.attend_decode(q, *c.args(), scale=0.1)
+    ctx = paged.context(DEV)
+    assert paged.context("cuda:0") is ctx
+    ctx.close()
+    ctx.close()
+    got = paged.attend_decode(q, *c.args(), scale=0.1)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert paged.context(DEV) is not ctx
+    paged.context(DEV).sync()
+
+
+def test_threads_and_streams_at_once():
+    """Four threads, each with its own stream, and two that share one: splits and
+    joins of one stream do not touch another's."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([3000, 700, 64, 1], 2, 128, 32, BF16)
+    start = torch.tensor([0, 8, 16, 24, 25], dtype=torch.int32, device=DEV)
+    shared = torch.cuda.Stream()
+    streams = [torch.cuda.Stream() for _ in range(4)] + [shared, shared]
+    qd = [queries(4, 8, 128, BF16, i, False) for i in range(6)]
+    qp = [queries(25, 8, 128, BF16, 50 + i, False) for i in range(6)]
+    torch.cuda.synchronize()
+
+    def once(i):
+        mass = torch.zeros(4, 2, 3000, device=DEV)
+        a = paged.attend_decode(qd[i], *c.args(), scale=0.1, mass=mass)
+        b = paged.attend_prompt(qp[i], start, 8, *c.args(), scale=0.1, mass=mass)
+        return (*a, *b, mass)
+
+    want = [once(i) for i in range(6)]
+    torch.cuda.synchronize()
+    wrong, contexts = [], set()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(streams[i]):
+                for _ in range(30):
+                    got = once(i)
+                    if not all(torch.equal(x, y) for x, y in zip(got, want[i])):
+                        wrong.append(i)
+            contexts.add(id(paged.context(DEV)))
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and len(contexts) == 1
+    paged.context(DEV).sync()
+
+
+def test_a_graph_outlives_the_thread_that_captured_it():
+    """Its kernels use the workspace of the stream, which is still there."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([4000, 33], 2, 128, 16, F16)
+    q = queries(2, 4, 128, F16, 0, False)
+    want, _ = paged.attend_decode(q, *c.args(), scale=0.1)
+    torch.cuda.synchronize()
+    made = {}
+
+    def capture():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            paged.attend_decode(q, *c.args(), scale=0.1)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out, _ = paged.attend_decode(q, *c.args(), scale=0.1)
+        made.update(graph=g, out=out, stream=s)
+
+    t = threading.Thread(target=capture)
+    t.start()
+    t.join()
+    for _ in range(3):
+        made["out"].zero_()
+        made["graph"].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(made["out"], want)
