@@ -8,8 +8,9 @@ runs a synthetic model (4B widths, few layers) and prints what it did.  The
 projections are QLinear layers over the same Q4_K weights as the decode engines
 (Gemma3Block::forward_cached, src/transformer4.rs:1954-1964); attention and
 caches are rich_triplet_b200.paged; norms, RoPE and the gate are torch
-operations.  Everything runs on the context's stream.  Without eviction and
-with no first tokens its logits are the engine's (CudaDecodeContext).
+operations.  A step runs on the context's stream, after the work of the caller's
+current stream, which waits for it.  Without eviction and with no first tokens
+its logits are the engine's (CudaDecodeContext).
 """
 
 import argparse
@@ -81,9 +82,16 @@ class PagedGemma3:
     def step(self, tokens):
         """One step for every sequence: tokens[b] is a list of new token ids (one
         each: a decode step; else a prompt step).  Returns the logits of each
-        sequence's last new token ([sequences, vocab] f32, on the device)."""
+        sequence's last new token ([sequences, vocab] f32, on the device), for use
+        on the caller's current stream."""
+        caller = torch.cuda.current_stream(self.stream.device)
+        self.stream.wait_stream(caller)
         with torch.cuda.stream(self.stream):
-            return self._step(tokens)
+            logits = self._step(tokens)
+        # the head's product may still run when the host gets here
+        caller.wait_stream(self.stream)
+        logits.record_stream(caller)
+        return logits
 
     def _step(self, tokens):
         cfg, D = self.cfg, self.cfg.head_dim
@@ -155,8 +163,7 @@ def main(argv=None):
     torch.cuda.synchronize()
     t1 = time.perf_counter()
     for _ in range(a.steps):
-        with torch.cuda.stream(model.stream):
-            tok = logits.argmax(-1).tolist()
+        tok = logits.argmax(-1).tolist()
         for o, t in zip(out, tok):
             o.append(t)
         logits = model.step([[t] for t in tok])

@@ -1,0 +1,46 @@
+"""Edges of Gemma 3 over paged caches (rich_triplet_b200.paged_model): streams,
+refused steps, errors reported by kernels."""
+
+import pytest
+import torch
+
+from rich_triplet_b200.model import Config4, synth_gemma3
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def tiny():
+    cfg = Config4.tiny()
+    return cfg, synth_gemma3(cfg, seed=1234)
+
+
+def test_logits_are_complete_on_the_callers_stream(tiny):
+    """The head's product is held back on the model's stream; the caller reads the
+    logits on its own, without a synchronisation, and writes into them."""
+    from rich_triplet_b200.paged_model import PagedGemma3
+
+    cfg, w = tiny
+    held = torch.randn(4096, 4096, device="cuda") * 1e-3
+    models = [PagedGemma3(w, 2, 32, page_size=8, dtype=torch.float16) for _ in range(2)]
+    linear = models[1]._linear
+
+    def late(layer, x):
+        if layer is models[1].head:
+            y = held
+            for _ in range(30):
+                y = y @ held
+            x = x + y.sum() * 0
+        return linear(layer, x)
+
+    models[1]._linear = late
+    side = torch.cuda.Stream()
+    for stream in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(stream):
+            want = models[0].step([[3, 4, 5], [6]])
+            torch.cuda.synchronize()
+            got = models[1].step([[3, 4, 5], [6]])
+            seen = got.clone()
+            got.zero_()
+        torch.cuda.synchronize()
+        assert torch.equal(seen, want) and not torch.equal(seen, got)
