@@ -36,6 +36,7 @@ class PagedGemma3:
         self.ctx = ctx or Context(0)
         self.stream = torch.cuda.ExternalStream(self.ctx.stream_ptr)
         self.sinks, self.budget, self.recent, self.page_size, self.dtype = sinks, budget, recent, page_size, dtype
+        self.max_len = max_len
         H, D, F = cfg.hidden_size, cfg.head_dim, cfg.intermediate_size
         nq, nkv = cfg.num_attention_heads, cfg.num_key_value_heads
         shapes = {"q": (nq * D, H), "k": (nkv * D, H), "v": (nkv * D, H), "o": (H, nq * D), "gate": (F, H), "up": (F, H),
@@ -99,10 +100,15 @@ class PagedGemma3:
         counts = [len(t) for t in tokens]
         if len(tokens) != len(self.position) or min(counts) < 1:
             raise ValueError(f"PagedGemma3.step: at least one token for each of {len(self.position)} sequences")
+        flat = np.concatenate(tokens).astype(np.int64)
+        if flat.min() < 0 or flat.max() >= cfg.vocab_size:
+            raise ValueError(f"PagedGemma3.step: tokens from {flat.min()} to {flat.max()}, vocabulary of {cfg.vocab_size}")
+        if max(p + c for p, c in zip(self.position, counts)) > self.max_len:
+            raise ValueError(f"PagedGemma3.step: {counts} tokens after {self.position} pass position {self.max_len}")
         decode = max(counts) == 1
         starts = np.concatenate([[0], np.cumsum(counts)])
         q_start = None if decode else torch.tensor(starts, dtype=torch.int32).cuda()
-        ids = torch.tensor(np.concatenate(tokens).astype(np.int64)).cuda()
+        ids = torch.tensor(flat).cuda()
         at = torch.tensor(np.concatenate([np.arange(p, p + c) for p, c in zip(self.position, counts)])).cuda()
         for c in self.caches:
             if c is not None:

@@ -44,3 +44,26 @@ def test_logits_are_complete_on_the_callers_stream(tiny):
             got.zero_()
         torch.cuda.synchronize()
         assert torch.equal(seen, want) and not torch.equal(seen, got)
+
+
+def test_tokens_and_positions_out_of_range_are_refused(tiny):
+    """Both index device tensors: refused on the host, and nothing has changed."""
+    from rich_triplet_b200.paged_model import PagedGemma3
+
+    cfg, w = tiny
+    model = PagedGemma3(w, 2, 16, page_size=8, dtype=torch.float16)
+    other = PagedGemma3(w, 2, 16, page_size=8, dtype=torch.float16)
+    for m in (model, other):
+        m.step([[1, 2, 3], [4]])
+    for bad in ([[cfg.vocab_size], [0]], [[0], [-1]], [[0], [5, 10 ** 12]]):
+        with pytest.raises(ValueError, match="vocabulary"):
+            model.step(bad)
+    with pytest.raises(ValueError, match="pass position 16"):
+        model.step([[1] * 14, [1]])
+    with pytest.raises(ValueError, match="at least one token"):
+        model.step([[1], []])
+    assert model.position == [3, 1]
+    tok = [[5], [6]]
+    assert torch.equal(model.step(tok), other.step(tok))
+    model.step([[1] * 12, [1]])  # up to the last position
+    assert model.position == [16, 3]
