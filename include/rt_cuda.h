@@ -511,7 +511,8 @@ int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_rows* row
  * rt_paged_decode: one token per sequence, at its last position; q_start must
  * be NULL and rows == num_seqs.  rt_paged_prompt: rows q_start[b] ..
  * q_start[b + 1] - 1 are the last tokens of sequence b; max_new bounds every
- * sequence's count (tokens beyond it are not computed); over an f32 cache rows
+ * sequence's count (tokens beyond it are not computed, nor those of a sequence
+ * whose q_start is negative, nor rows beyond `rows`); over an f32 cache rows
  * times query heads to a KV head are at most 2^25.
  * scratch: rt_paged_scratch bytes of device memory, 256-byte aligned (NULL
  * when that is 0), which the call's work uses until it has run. */

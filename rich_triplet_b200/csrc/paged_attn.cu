@@ -23,6 +23,7 @@ __global__ void __launch_bounds__(128) paged_mass32_kernel(const PagedKv kv, con
     const int len = kv.len(b);
     if (j >= len || j >= a.mass_cap) return;
     const int64_t first = a.q_start[b], all = a.q_start[b + 1] - first;
+    if (first < 0) return;
     const int64_t count = min(min(all, static_cast<int64_t>(a.max_new)), a.rows - first);
     const int64_t t0 = len - all;  // position of the first new token
     const int64_t off = kv.row(b, j);

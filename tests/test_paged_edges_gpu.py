@@ -192,3 +192,33 @@ def test_a_graph_outlives_the_thread_that_captured_it():
         made["graph"].replay()
         torch.cuda.synchronize()
         assert torch.equal(made["out"], want)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_row_starts_outside_the_rows(dtype):
+    """q_start is read on the device: sequences that begin before row 0 or end
+    past the last row read and write no row that is not there."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([40, 50, 60], 2, 64, 16, dtype)
+    room = torch.full((30, 4, 64), 5.0, dtype=dtype, device=DEV)
+    q = queries(30, 4, 64, dtype, 0, False)[10:20]
+    out = room[10:20]
+    mass = torch.zeros(3, 2, 60, device=DEV)
+    for starts in ([-7, -2, 3, 10], [-9, 4, 4, 1000], [12, 15, 20, 25]):
+        room.fill_(5.0)
+        mass.zero_()
+        start = torch.tensor(starts, dtype=torch.int32, device=DEV)
+        _, lse = paged.attend_prompt(q, start, 10, *c.args(), scale=0.1, mass=mass, out=out)
+        assert (room[:10] == 5).all() and (room[20:] == 5).all()
+        for b in range(3):
+            first, end = starts[b], min(starts[b + 1], 10)
+            # token i of the starts[b + 1] - first ones is at position c.lens[b] - (starts[b + 1] - first) + i
+            rows = [r for r in range(max(0, first), end) if c.lens[b] - starts[b + 1] + r >= 0] if first >= 0 else []
+            assert abs(float(mass[b].sum()) - 4 * len(rows)) < 1e-2
+            assert torch.isfinite(lse[rows]).all()
+        k = torch.randn(10, 2, 64, device=DEV)
+        before = c.kp.clone()
+        paged.kv_append(c.kp, c.vp, k, k, c.table, c.lens_t, q_start=start)
+        c.kp.copy_(before)
+        c.vp.copy_(before)
