@@ -535,7 +535,8 @@ typedef struct {
     uint64_t scratch_bytes;
 } rt_paged_attn;
 /* Scratch bytes of a call with these arguments (no pointer is followed; mass
- * and lse only for whether they are NULL). */
+ * and lse only for whether they are NULL); RT_E_SHAPE for sizes that no call
+ * takes. */
 int rt_paged_scratch(const rt_paged_kv* kv, const rt_paged_attn* a, int32_t prompt, uint64_t* bytes);
 int rt_paged_decode(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_attn* a, void* stream);
 int rt_paged_prompt(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_attn* a, void* stream);

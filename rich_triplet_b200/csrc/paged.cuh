@@ -110,7 +110,7 @@ cudaError_t paged_append_launch(const PagedKv& kv, const PagedRows& r, cudaStrea
 // call leaves them zero), then partial results.
 size_t paged_workspace_bytes(int num_sms);
 size_t paged_counter_bytes(int num_sms);
-size_t paged_decode_scratch(const PagedKv& kv, const PagedAttn& a);
+uint64_t paged_decode_scratch(const PagedKv& kv, const PagedAttn& a);
 cudaError_t paged_decode_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, void* scratch, int num_sms,
                                 cudaStream_t s);
 cudaError_t paged_prompt32_launch(const PagedKv& kv, const PagedAttn& a, void* workspace, int num_sms, cudaStream_t s);

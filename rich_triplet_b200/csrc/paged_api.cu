@@ -40,6 +40,10 @@ bool strides_ok(int esize, S... s) {
     return ((s >= 0 && s * esize % 16 == 0) && ...);
 }
 
+constexpr int64_t kMaxPositions = INT32_MAX - 256;  // of a sequence
+
+bool page_size_ok(int page_size) { return page_size >= 8 && page_size <= 256 && (page_size & (page_size - 1)) == 0; }
+
 // Whether n x m rows of `len` elements, at i * si + j * sj, lie apart: rows of
 // one index hold those of the other between them.
 bool apart(int64_t n, int64_t si, int64_t m, int64_t sj, int64_t len) {
@@ -57,7 +61,7 @@ int make_kv(rt_ctx* ctx, const char* who, const rt_paged_kv* in, rt::PagedKv* ou
     if (type < 0) return fail(ctx, RT_E_FORMAT, "%s: cache format %d is not f32, f16 or bf16", who, in->fmt);
     if (in->head_dim != 64 && in->head_dim != 128 && in->head_dim != 256)
         return fail(ctx, RT_E_SHAPE, "%s: head_dim %d is not 64, 128 or 256", who, in->head_dim);
-    if (in->page_size < 8 || in->page_size > 256 || (in->page_size & (in->page_size - 1)))
+    if (!page_size_ok(in->page_size))
         return fail(ctx, RT_E_SHAPE, "%s: page_size %d is not a power of two in 8..256", who, in->page_size);
     if (in->kv_heads < 1 || in->kv_heads > 65535)
         return fail(ctx, RT_E_SHAPE, "%s: kv_heads %d out of range", who, in->kv_heads);
@@ -66,7 +70,7 @@ int make_kv(rt_ctx* ctx, const char* who, const rt_paged_kv* in, rt::PagedKv* ou
     if (in->num_seqs < 0 || in->num_seqs > 65535)
         return fail(ctx, RT_E_SHAPE, "%s: num_seqs %d out of range (0..65535)", who, in->num_seqs);
     if (in->table_width < 0 || in->table_stride < 0 ||
-        static_cast<int64_t>(in->table_width) * in->page_size > INT32_MAX - 256 ||
+        static_cast<int64_t>(in->table_width) * in->page_size > kMaxPositions ||
         static_cast<int64_t>(in->table_width) * in->page_size * in->num_seqs > (int64_t{1} << 44))
         return fail(ctx, RT_E_SHAPE, "%s: page table of width %d, row stride %lld", who, in->table_width,
                     static_cast<long long>(in->table_stride));
@@ -130,7 +134,8 @@ int make_attn(rt_ctx* ctx, const char* who, const rt_paged_kv* kv, const rt_page
 // The prompt mass pass reads every row's lse: room for it when the caller takes none.
 uint64_t scratch_need(const rt::PagedKv& kv, const rt::PagedAttn& a, bool prompt) {
     if (!prompt) return rt::paged_decode_scratch(kv, a);
-    return a.mass && !a.lse ? (static_cast<uint64_t>(a.rows) * a.nq * 4 + 255) / 256 * 256 : 0;
+    if (!a.mass || a.lse) return 0;
+    return a.rows > INT64_MAX / 8 / a.nq ? UINT64_MAX : (static_cast<uint64_t>(a.rows) * a.nq * 4 + 255) / 256 * 256;
 }
 
 // The stream's workspace, made on first use.
@@ -216,7 +221,9 @@ int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* in, const rt_paged_rows* r, 
 
 int rt_paged_scratch(const rt_paged_kv* in, const rt_paged_attn* at, int32_t prompt, uint64_t* bytes) {
     if (!in || !at || !bytes) return RT_E_INVAL;
-    if (in->page_size < 1 || at->rows < 0 || in->table_width < 0 || at->num_heads < 1 || at->window < 0 || at->sinks < 0)
+    if (!page_size_ok(in->page_size) || in->table_width < 0 ||
+        static_cast<int64_t>(in->table_width) * in->page_size > kMaxPositions || at->rows < 0 || at->num_heads < 1 ||
+        at->window < 0 || at->sinks < 0)
         return RT_E_SHAPE;
     rt::PagedKv kv = {};
     rt::PagedAttn a = {};
@@ -229,7 +236,7 @@ int rt_paged_scratch(const rt_paged_kv* in, const rt_paged_attn* at, int32_t pro
     a.mass = at->mass;
     a.lse = at->lse;
     *bytes = scratch_need(kv, a, prompt != 0);
-    return RT_OK;
+    return *bytes == UINT64_MAX ? RT_E_SHAPE : RT_OK;
 }
 
 int rt_paged_decode(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_attn* a, void* stream) {

@@ -56,9 +56,12 @@ static int64_t score_stride(const PagedKv& kv, const PagedAttn& a) {
     return a.window > 0 ? std::min<int64_t>(cap, static_cast<int64_t>(a.window) + a.sinks) : cap;
 }
 
-size_t paged_decode_scratch(const PagedKv& kv, const PagedAttn& a) {
+// All ones where it passes 2^62 bytes.
+uint64_t paged_decode_scratch(const PagedKv& kv, const PagedAttn& a) {
     if (!a.mass) return 0;
-    const size_t rows = static_cast<size_t>(a.rows) * a.nq;
+    const int64_t each = static_cast<int64_t>(sizeof(float2)) + score_stride(kv, a) * static_cast<int64_t>(sizeof(float));
+    if (a.rows > (int64_t{1} << 62) / a.nq / each) return UINT64_MAX;
+    const uint64_t rows = static_cast<uint64_t>(a.rows) * a.nq;
     return (rows * sizeof(float2) + 255) / 256 * 256 + (rows * score_stride(kv, a) * sizeof(float) + 255) / 256 * 256;
 }
 

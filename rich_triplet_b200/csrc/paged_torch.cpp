@@ -252,8 +252,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
             t.mass_seq_stride = m->stride(0);
             t.mass_head_stride = m->stride(1);
             uint64_t need = 0;
-            if (!done(rt_paged_scratch(&c.kv, &t, prompt, &need), nullptr)) return nullptr;
-            if (need) {
+            if (rt_paged_scratch(&c.kv, &t, prompt, &need) == RT_OK && need) {  // else the call below refuses
                 // freed when this call returns: only later work of this stream takes its place
                 scratch = at::empty({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
                 t.scratch = scratch.data_ptr();

@@ -1,6 +1,11 @@
 """Edges of the paged cache's host side: contexts, size limits of the C entry
 points, bookkeeping of pages.  No GPU."""
 
+import ctypes
+import os
+import subprocess
+import sys
+
 import pytest
 import torch  # noqa: F401
 
@@ -13,3 +18,55 @@ def test_forget_and_sync_without_a_context():
     assert paged._ext.sync(5) is None
     with pytest.raises(TypeError):
         paged._ext.sync()
+
+
+class Kv(ctypes.Structure):
+    """rt_paged_kv"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("slot_stride", ctypes.c_int64), ("num_pages", ctypes.c_int64),
+                ("fmt", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("table_width", ctypes.c_int32), ("num_seqs", ctypes.c_int32), ("lens", ctypes.c_void_p)]
+
+
+class Attn(ctypes.Structure):
+    """rt_paged_attn"""
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_row_stride", ctypes.c_int64),
+                ("q_head_stride", ctypes.c_int64), ("out_row_stride", ctypes.c_int64),
+                ("out_head_stride", ctypes.c_int64), ("lse", ctypes.c_void_p), ("lse_row_stride", ctypes.c_int64),
+                ("rows", ctypes.c_int64), ("num_heads", ctypes.c_int32), ("window", ctypes.c_int32),
+                ("sinks", ctypes.c_int32), ("max_new", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("mass_cap", ctypes.c_int32), ("q_start", ctypes.c_void_p), ("mass", ctypes.c_void_p),
+                ("mass_seq_stride", ctypes.c_int64), ("mass_head_stride", ctypes.c_int64),
+                ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_uint64)]
+
+
+SCRATCH = """
+import ctypes, sys
+sys.path[:0] = {path!r}
+import test_paged_edges_cpu as t
+from rich_triplet_b200._lib import lib
+for kv, attn in {calls!r}:
+    kv, a, n = t.Kv(**kv), t.Attn(**attn), ctypes.c_uint64(7)
+    print(lib().rt_paged_scratch(ctypes.byref(kv), ctypes.byref(a), 0, ctypes.byref(n)), n.value)
+"""
+
+
+def test_scratch_of_any_sizes_answers():
+    """In a process of its own: sizes that no call takes get an answer, not a hang."""
+
+    def call(page, width, rows, heads):
+        return (dict(fmt=0, kv_heads=2, head_dim=64, page_size=page, table_width=width, num_seqs=3),
+                dict(rows=rows, num_heads=heads, mass=16, mass_cap=9))
+
+    bad = [call(page, 5, 3, 4) for page in (2 ** 30 + 1, 2 ** 31 - 1, 512, 24, 0, -8)]
+    bad += [call(256, 2 ** 31 - 1, 3, 4), call(256, -1, 3, 4), call(16, 5, -1, 4), call(16, 5, 3, 0)]
+    bad += [call(256, 2 ** 23 - 1, 2 ** 27, 2 ** 20)]  # the product passes 64 bits
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = SCRATCH.format(path=[here, os.path.dirname(here)], calls=[call(16, 5, 3, 4)] + bad)
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=60)
+    assert got.returncode == 0, got.stderr
+    got = [tuple(int(x) for x in line.split()) for line in got.stdout.splitlines()]
+    # 3 x 4 rows of 5 pages of 16 positions, and their maxima and sums
+    assert got[0] == (0, 256 + 3840)
+    assert [status for status, _ in got[1:]] == [-4] * len(bad)
