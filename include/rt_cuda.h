@@ -452,7 +452,8 @@ int rt_qwen35_logits_device(rt_qwen35* eng, const float** out);
  * freed pages may stay in the table.
  *
  * Limits: fmt RT_FMT_F32, RT_FMT_F16 or RT_FMT_BF16; head_dim 64, 128 or 256;
- * page_size a power of two in 8..256; pools, queries, outputs and rows
+ * page_size a power of two in 8..256; at most 2^31 - 257 positions in a table
+ * row (and in an eviction's budget and mass row); pools, queries, outputs and rows
  * 16-byte aligned, all their strides multiples of 16 bytes.
  *
  * Workspace: the context keeps one fixed workspace per stream, made by the

@@ -254,6 +254,9 @@ int rt_paged_evict(rt_ctx* ctx, const rt_paged_kv* in, const rt_paged_evict_args
     if (int rc = make_kv(ctx, who, in, &kv); rc != RT_OK) return rc;
     if (e->budget < 1 || e->sinks < 0 || e->recent < 0 || static_cast<int64_t>(e->sinks) + e->recent > e->budget)
         return fail(ctx, RT_E_INVAL, "%s: sinks %d + recent %d must lie in 0..budget %d", who, e->sinks, e->recent, e->budget);
+    if (e->budget > kMaxPositions || e->mass_cap > kMaxPositions)
+        return fail(ctx, RT_E_SHAPE, "%s: budget %d, mass_cap %d: at most %lld positions", who, e->budget, e->mass_cap,
+                    static_cast<long long>(kMaxPositions));
     if (e->mass_cap < 0 || e->mass_seq_stride < 0 || e->mass_head_stride < 0)
         return fail(ctx, RT_E_SHAPE, "%s: negative mass size or stride", who);
     if (!apart(in->num_seqs, e->mass_seq_stride, in->kv_heads, e->mass_head_stride, e->mass_cap))

@@ -140,9 +140,12 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedKv kv
     float* mout = e.mass_out + b * e.mass_seq + h * e.mass_head;
     int32_t* kept = e.kept + (static_cast<int64_t>(b) * kv.nkv + h) * e.budget;
     if (h == 0 && tid == 0) e.new_lens[b] = n;
-    const int blocks = (len + kBlock - 1) / kBlock;
+    const int blocks = static_cast<int>((static_cast<uint32_t>(len) + kBlock - 1) / kBlock);
     const bool all = len <= e.budget;
-    auto position = [&](int blk, int i) { return blk * kBlock + warp * 256 + i * 32 + lane; };
+    // (the last block may end past 2^31, where a position counts as past the end)
+    auto position = [&](int blk, int i) {
+        return static_cast<int>(min(static_cast<uint32_t>(blk) * kBlock + warp * 256 + i * 32 + lane, 0x7FFFFFFFu));
+    };
     auto load_keys = [&](int blk, uint32_t(&k)[kKeysEach]) {  // all loads before the first use
         float x[kKeysEach];
 #pragma unroll
@@ -258,8 +261,8 @@ __global__ void __launch_bounds__(kThreads) paged_select_kernel(const PagedKv kv
             at += __popc(keep[i]);
         }
     });
-    for (int i = n + tid; i < e.budget; i += kThreads) kept[i] = -1;
-    for (int i = n + tid; i < e.mass_cap; i += kThreads) mout[i] = 0.f;
+    for (int64_t i = n + tid; i < e.budget; i += kThreads) kept[i] = -1;
+    for (int64_t i = n + tid; i < e.mass_cap; i += kThreads) mout[i] = 0.f;
 }
 
 // A warp moves the K and V of eight kept rows (row bytes 16 CPR), their page
@@ -326,7 +329,7 @@ cudaError_t paged_evict_launch(const PagedKv& kv, const PagedEvict& e, cudaStrea
     else paged_select_kernel<1024, false><<<rows, 1024, 0, s>>>(kv, e);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
-    const dim3 grid((e.budget + 63) / 64, kv.nkv, kv.nseq);
+    const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(e.budget) + 63) / 64), kv.nkv, kv.nseq);
     switch (kv.D * (kv.type == kPagedF32 ? 4 : 2) / 16) {
         case 8: return rt_launch(paged_gather_kernel<8>, grid, 256, 0, s, true, kv, e);
         case 16: return rt_launch(paged_gather_kernel<16>, grid, 256, 0, s, true, kv, e);

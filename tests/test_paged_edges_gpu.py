@@ -222,3 +222,24 @@ def test_row_starts_outside_the_rows(dtype):
         paged.kv_append(c.kp, c.vp, k, k, c.table, c.lens_t, q_start=start)
         c.kp.copy_(before)
         c.vp.copy_(before)
+
+
+def test_evict_budget_at_the_limit():
+    """Loops over a row of nearly 2^31 entries end at its end (the kept positions
+    take 8.6 GB)."""
+    from rich_triplet_b200 import paged
+
+    most = 2 ** 31 - 257
+    c = Cache([50, 0], 1, 64, 256, F16, spare=3)
+    dst = torch.full((1, 2 ** 23 - 1), int(c.free[0]), dtype=torch.int32, device=DEV)
+    mass = torch.rand(1, 1, 50, device=DEV)
+    one = (c.kp, c.vp, c.table[:1], c.lens_t[:1])
+    kept, lens, out = paged.kv_evict(*one, mass, dst, budget=most)
+    assert lens.tolist() == [50] and torch.equal(out, mass)
+    assert kept[0, 0, :50].tolist() == list(range(50))
+    assert int(kept[0, 0, 50:].max()) == -1 and int(kept[0, 0, 50:].min()) == -1
+    del kept
+    torch.cuda.empty_cache()
+    dst = torch.zeros(1, 2 ** 23, dtype=torch.int32, device=DEV)
+    refused(RtError, "at most 2147483391 positions", paged.kv_evict, *one, mass, dst, budget=most + 1)
+    torch.cuda.empty_cache()
