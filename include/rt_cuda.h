@@ -507,7 +507,8 @@ int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_rows* row
  * visible j < mass_cap: the running total that rt_paged_evict ranks by.
  * Results do not depend on launch order: every sum has a fixed order.  Rows of
  * out, and rows of mass, that overlap one another (a stride of 0, say) are
- * refused.
+ * refused; so is an out that shares values with q in rt_paged_prompt with mass,
+ * whose second pass reads q again.
  *
  * rt_paged_decode: one token per sequence, at its last position; q_start must
  * be NULL and rows == num_seqs.  rt_paged_prompt: rows q_start[b] ..

@@ -56,6 +56,25 @@ bool apart(int64_t n, int64_t si, int64_t m, int64_t sj, int64_t len) {
     return n <= 0 || m <= 0 || len <= 0 || nested(n, si, m, sj) || nested(m, sj, n, si);
 }
 
+// Whether a value of q is also one of out.  (Exact for equal strides; for
+// unequal ones two ranges that meet count as shared.)
+bool q_meets_out(const rt_paged_attn* a, int esize, int D) {
+    auto span = [&](int64_t row, int64_t head) { return ((a->rows - 1) * row + (a->num_heads - 1) * head + D) * esize; };
+    const intptr_t q = reinterpret_cast<intptr_t>(a->q), out = reinterpret_cast<intptr_t>(a->out);
+    if (a->rows < 1 || q + span(a->q_row_stride, a->q_head_stride) <= out ||
+        out + span(a->out_row_stride, a->out_head_stride) <= q)
+        return false;
+    const int64_t row = a->rows > 1 ? a->q_row_stride : 0, head = a->num_heads > 1 ? a->q_head_stride : 0;
+    if ((a->rows > 1 && row != a->out_row_stride) || (a->num_heads > 1 && head != a->out_head_stride)) return true;
+    for (int64_t h = 1 - a->num_heads; h < a->num_heads; ++h) {
+        const int64_t d = (out - q) / esize - h * head;  // what row differences have to make up
+        const int64_t r = row ? d / row : 0;
+        for (int64_t i = r - 1; i <= r + 1; ++i)
+            if (i > -a->rows && i < a->rows && d - i * row > -D && d - i * row < D) return true;
+    }
+    return false;
+}
+
 int make_kv(rt_ctx* ctx, const char* who, const rt_paged_kv* in, rt::PagedKv* out) {
     const int type = paged_type(in->fmt);
     if (type < 0) return fail(ctx, RT_E_FORMAT, "%s: cache format %d is not f32, f16 or bf16", who, in->fmt);
@@ -122,6 +141,8 @@ int make_attn(rt_ctx* ctx, const char* who, const rt_paged_kv* kv, const rt_page
     if (in->lse && in->lse_row_stride < in->num_heads) return fail(ctx, RT_E_SHAPE, "%s: lse rows overlap", who);
     if (in->mass && (in->mass_cap < 0 || in->mass_seq_stride < 0 || in->mass_head_stride < 0))
         return fail(ctx, RT_E_SHAPE, "%s: negative mass size or stride", who);
+    if (prompt && in->mass && q_meets_out(in, esize, kv->head_dim))
+        return fail(ctx, RT_E_INVAL, "%s: out overlaps q, which the totals read again", who);
     if (in->mass && !apart(kv->num_seqs, in->mass_seq_stride, kv->kv_heads, in->mass_head_stride, in->mass_cap))
         return fail(ctx, RT_E_SHAPE, "%s: the rows of mass overlap", who);
     *out = rt::PagedAttn{in->q, in->out, in->q_row_stride, in->q_head_stride, in->out_row_stride, in->out_head_stride,

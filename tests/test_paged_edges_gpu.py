@@ -243,3 +243,30 @@ def test_evict_budget_at_the_limit():
     dst = torch.zeros(1, 2 ** 23, dtype=torch.int32, device=DEV)
     refused(RtError, "at most 2147483391 positions", paged.kv_evict, *one, mass, dst, budget=most + 1)
     torch.cuda.empty_cache()
+
+
+def test_prompt_totals_read_the_queries_after_the_outputs():
+    """An output over the queries is refused where the totals need them again; one
+    beside them in the same rows is taken."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([40, 9], 2, 64, 16, BF16)
+    start = torch.tensor([0, 20, 26], dtype=torch.int32, device=DEV)
+    wide = torch.randn(26, 10, 64, device=DEV).to(BF16)
+    q = wide[:, 1:5]
+    mass = torch.zeros(2, 2, 40, device=DEV)
+    o, z = paged.attend_prompt(q.clone(), start, 20, *c.args(), scale=0.1, mass=mass)
+    for out in (q, wide[:, 2:6], wide[:, :8:2]):
+        refused(RtError, "out overlaps q", paged.attend_prompt, q, start, 20, *c.args(), scale=0.1, mass=mass.clone(),
+                out=out)
+    for q2, out in ((q, wide[:, 5:9]), (wide[:, :8:2], wide[:, 1:9:2]), (wide.view(260, 64)[:104].view(26, 4, 64),
+                                                                       wide.view(260, 64)[104:208].view(26, 4, 64))):
+        q2.copy_(torch.randn(26, 4, 64, device=DEV))
+        got = [torch.zeros_like(mass) for _ in range(2)]
+        want, _ = paged.attend_prompt(q2.clone(), start, 20, *c.args(), scale=0.1, mass=got[0])
+        paged.attend_prompt(q2, start, 20, *c.args(), scale=0.1, mass=got[1], out=out)
+        assert torch.equal(out, want) and torch.equal(got[0], got[1])
+    # without totals, and for single tokens, every query is read before an output is written
+    x = wide[:, 1:5].clone()
+    assert torch.equal(paged.attend_prompt(x, start, 20, *c.args(), scale=0.1, out=x)[0],
+                       paged.attend_prompt(wide[:, 1:5], start, 20, *c.args(), scale=0.1)[0])
