@@ -497,7 +497,10 @@ int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* kv, const rt_paged_rows* row
  * j > t - window) or among the first `sinks`.
  *   out[r][h] = sum_j softmax_j(scale * q . k_j) v_j   (cache's type)
  *   lse[r][h] = log sum_j exp(scale * q . k_j)          (f32; NULL: not wanted)
- * A token that sees nothing (an empty sequence) gets out 0 and lse -inf.
+ * A token that sees nothing (an empty sequence), or whose visible scores are all
+ * -inf, gets out 0 and lse -inf.  NaN in its query or in a key that it sees makes
+ * its out and lse NaN; infinite elements may do so too (a score of +inf does, and
+ * over an f32 cache, whose values are multiplied in two parts, any infinity).
  * Rows that no token of the call sees may hold anything.  A value row that some
  * token sees must be finite: of rt_paged_prompt's tokens, those computed in one
  * tile with it (128 rows of token and head) multiply it by a weight of zero.

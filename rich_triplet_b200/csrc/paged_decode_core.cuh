@@ -36,6 +36,9 @@
 // 5.5 TB/s.  64 windows of 1028: 46 us, 5.8 TB/s.  301 positions: 9.2 us, six
 // dependent trips to memory (length, page, rows, part, counter, parts).
 //
+// A state has seen no weight where its sum is 0, whatever its maximum: NaN scores
+// do not move the maximum, but their NaN is in the sum and in the output.
+//
 // The maximum is only moved when a score exceeds it by more than 8 (powers of
 // two), so weights stay below 2^8 and most tiles rescale nothing.
 #pragma once
@@ -694,12 +697,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                 A.w += v.w * f;
             }
             if (whole) {
-                const float inv = M == -INFINITY ? 0.f : 1.f / L;
+                const float inv = L == 0.f ? 0.f : 1.f / L;
                 const int64_t row = row_at(g);
                 const int head = head_at(g);
                 store4(static_cast<T*>(a.out) + row * a.out_row + head * a.out_head + d, A, inv);
                 if (d == 0) {
-                    if (a.lse) a.lse[row * a.lse_row + head] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
+                    if (a.lse) a.lse[row * a.lse_row + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
                     if (!FEW && wk.norm) wk.norm[row * a.nq + head] = make_float2(M, inv);
                 }
             } else {
@@ -740,11 +743,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                     }
                     L = warp_sum(L);
                     if (lane == 0) {
-                        const float inv = M == -INFINITY ? 0.f : 1.f / L;
+                        const float inv = L == 0.f ? 0.f : 1.f / L;
                         st[n * ncol + g].x = inv;
                         const int64_t row = row_at(g);
                         const int head = head_at(g);
-                        if (a.lse) a.lse[row * a.lse_row + head] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
+                        if (a.lse) a.lse[row * a.lse_row + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
                         if (!FEW && wk.norm) wk.norm[row * a.nq + head] = make_float2(M, inv);
                     }
                 }

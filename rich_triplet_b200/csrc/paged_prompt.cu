@@ -561,7 +561,8 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
         const int64_t item = bid;
         float* rec = wk.part + ((item * wk.nsplit + split) * NQ * kRows + r) * CS;
         T* out = static_cast<T*>(a.out) + (q_first + tok) * a.out_row + head * a.out_head;
-        const bool none = m == -INFINITY;
+        // no weight seen (NaN scores leave the maximum where it is, but not the sum)
+        const bool none = l == 0.f;
         const float inv = none ? 0.f : 1.f / l;
         if (ok && warp_live) {
 #pragma unroll 1
@@ -627,11 +628,11 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                             L += ml[s].y * f;
                             wgt[row * (kMaxSplit + 1) + s] = f;
                         }
-                    wgt[row * (kMaxSplit + 1) + kMaxSplit] = M == -INFINITY ? 0.f : 1.f / L;
+                    wgt[row * (kMaxSplit + 1) + kMaxSplit] = L == 0.f ? 0.f : 1.f / L;
                     const int rr = row0 + row, tk = rr / G;
                     if (a.lse)
                         a.lse[(q_first + tk) * a.lse_row + h * G + rr - tk * G] =
-                            M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
+                            L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945309f;
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory");
                 // eight float4 of the output a thread at a time, so that their loads overlap

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from rich_triplet_b200._lib import RtError
-from test_paged_gpu import BF16, DEV, F16, F32, Cache, queries
+from test_paged_gpu import BF16, DEV, F16, F32, Cache, close, is_visible, queries, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -270,3 +270,76 @@ def test_prompt_totals_read_the_queries_after_the_outputs():
     x = wide[:, 1:5].clone()
     assert torch.equal(paged.attend_prompt(x, start, 20, *c.args(), scale=0.1, out=x)[0],
                        paged.attend_prompt(wide[:, 1:5], start, 20, *c.args(), scale=0.1)[0])
+
+
+def check_beside_nan(dtype, nq, nkv, d, lens, new, bad, window=0, sinks=0):
+    """Prompt rows of which those in `bad` (row, head) have a NaN query: NaN there,
+    the definition elsewhere, totals NaN where such a token sees a position."""
+    from rich_triplet_b200 import paged
+
+    c = Cache(lens, nkv, d, 32, dtype)
+    starts = [sum(new[:i]) for i in range(len(new) + 1)]
+    q = queries(starts[-1], nq, d, dtype, 3, False)
+    for r, h in bad:
+        q[r, h, (r * 7 + h) % d] = float("nan")
+    mass = torch.zeros(len(lens), nkv, max(lens), device=DEV)
+    start = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    out, lse = paged.attend_prompt(q, start, max(new), *c.args(), scale=d ** -0.5, window=window, sinks=sinks, mass=mass)
+    for b, (n, m) in enumerate(zip(lens, new)):
+        t = torch.arange(n - m, n, device=DEV)
+        rows = slice(starts[b], starts[b + 1])
+        o, ob, z, zb, _, _ = reference(c, b, q[rows], t, d ** -0.5, window, sinks)
+        nan = torch.isnan(z)
+        assert nan.any() == any(starts[b] <= r < starts[b + 1] for r, _ in bad)
+        assert torch.equal(torch.isnan(lse[rows]), nan)
+        assert torch.equal(torch.isnan(out[rows]), nan[..., None].expand(-1, -1, d))
+        close(lse[rows][~nan], z[~nan], zb[~nan], f"lse of sequence {b}")
+        close(out[rows][~nan], o[~nan], ob[~nan], f"out of sequence {b}")
+
+
+@pytest.mark.parametrize("dtype,nq,nkv,d", [(BF16, 8, 4, 256), (F16, 4, 2, 128), (BF16, 8, 1, 64), (F32, 4, 2, 64),
+                                            (F16, 3, 1, 128)])
+def test_prompt_queries_with_nan(dtype, nq, nkv, d):
+    # a long prompt, a short one on a filled cache (its walk is split), one without NaN
+    check_beside_nan(dtype, nq, nkv, d, [300, 2000, 70], [300, 5, 9], [(0, 0), (100, 1), (131, 2), (301, 0)])
+    check_beside_nan(dtype, nq, nkv, d, [300, 700], [300, 8], [(40, 0), (305, 1)], window=50, sinks=3)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 256), (F16, 128), (F32, 64)])
+def test_prompt_keys_with_nan_or_infinity(dtype, d):
+    """Tokens that see such a key get NaN, the earlier ones of the same tile do not."""
+    from rich_triplet_b200 import paged
+
+    for value in (float("nan"), float("inf")):
+        c = Cache([200], 2, d, 16, dtype)
+        c.kp[c.table[0, 150 // 16].long(), 1, 150 % 16, 5] = value
+        q = queries(200, 4, d, dtype, 0, False)
+        q[:, :, 5] = q[:, :, 5].abs() + 0.5  # infinity times zero or a negative number is another case
+        start = torch.tensor([0, 200], dtype=torch.int32, device=DEV)
+        mass = torch.zeros(1, 2, 200, device=DEV)
+        out, lse = paged.attend_prompt(q, start, 200, *c.args(), scale=0.1, mass=mass)
+        assert torch.isnan(out[150:, 2:]).all() and torch.isfinite(out[:150]).all() and torch.isfinite(out[:, :2]).all()
+        assert torch.isfinite(lse[:150]).all() and torch.isfinite(lse[:, :2]).all() and not torch.isfinite(lse[150:, 2:]).any()
+        assert torch.isfinite(mass[:, 0]).all() and torch.isnan(mass[:, 1, :151]).all()
+
+
+@pytest.mark.parametrize("dtype,nq,nkv,d", [(BF16, 8, 4, 256), (F16, 16, 1, 128), (F32, 4, 2, 64), (F16, 8, 1, 64)])
+def test_decode_queries_with_nan(dtype, nq, nkv, d):
+    from rich_triplet_b200 import paged
+
+    lens = [1, 5, 300, 20000]
+    c = Cache(lens, nkv, d, 32, dtype)
+    q = queries(4, nq, d, dtype, 3, False)
+    q[0, 0], q[2, nq - 1, 3], q[3, 1, 9] = float("nan"), float("nan"), float("nan")
+    mass = torch.zeros(4, nkv, 20000, device=DEV)
+    out, lse = paged.attend_decode(q, *c.args(), scale=d ** -0.5, mass=mass)
+    for b, n in enumerate(lens):
+        o, ob, z, zb, w, wb = reference(c, b, q[b:b + 1], torch.tensor([n - 1], device=DEV), d ** -0.5, 0, 0)
+        nan = torch.isnan(z)
+        assert torch.equal(torch.isnan(lse[b:b + 1]), nan)
+        assert torch.equal(torch.isnan(out[b:b + 1]), nan[..., None].expand(-1, -1, d))
+        close(lse[b:b + 1][~nan], z[~nan], zb[~nan], f"lse of sequence {b}")
+        close(out[b:b + 1][~nan], o[~nan], ob[~nan], f"out of sequence {b}")
+        touched = torch.isnan(w)
+        assert torch.equal(torch.isnan(mass[b, :, :n]), touched) and (mass[b, :, n:] == 0).all()
+        close(mass[b, :, :n][~touched], w[~touched], wb[~touched], f"mass of sequence {b}")
