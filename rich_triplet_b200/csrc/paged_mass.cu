@@ -31,6 +31,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "gemv.cuh"
@@ -306,19 +307,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[buf]);
                 }
-                if (masked) {
+                auto add = [&](auto with_mask) {
 #pragma unroll
-                    for (int e = 0; e < 64; ++e)
-                        if (c + e < c_see || c + e >= c_until) x[e] = -INFINITY;
-                }
-#pragma unroll
-                for (int e = 0; e < 64; e += 4) {
-                    const float4 z = *reinterpret_cast<const float4*>(rz + c + e);
-                    const float2 w0 = ffma2(make_float2(x[e], x[e + 1]), sc, make_float2(z.x, z.y));
-                    const float2 w1 = ffma2(make_float2(x[e + 2], x[e + 3]), sc, make_float2(z.z, z.w));
-                    part[0] = tc::add2(part[0], make_float2(tc::ex2(w0.x), tc::ex2(w0.y)));
-                    part[1] = tc::add2(part[1], make_float2(tc::ex2(w1.x), tc::ex2(w1.y)));
-                }
+                    for (int e = 0; e < 64; e += 4) {
+                        const float4 z = *reinterpret_cast<const float4*>(rz + c + e);
+                        float2 w0 = ffma2(make_float2(x[e], x[e + 1]), sc, make_float2(z.x, z.y));
+                        float2 w1 = ffma2(make_float2(x[e + 2], x[e + 3]), sc, make_float2(z.z, z.w));
+                        if constexpr (decltype(with_mask)::value) {
+                            // behind the log-sum, which is NaN where a row has a NaN
+                            auto see = [&](float v, int at) { return at < c_see || at >= c_until ? -INFINITY : v; };
+                            w0 = make_float2(see(w0.x, c + e), see(w0.y, c + e + 1));
+                            w1 = make_float2(see(w1.x, c + e + 2), see(w1.y, c + e + 3));
+                        }
+                        part[0] = tc::add2(part[0], make_float2(tc::ex2(w0.x), tc::ex2(w0.y)));
+                        part[1] = tc::add2(part[1], make_float2(tc::ex2(w1.x), tc::ex2(w1.y)));
+                    }
+                };
+                if (masked) add(std::true_type());
+                else add(std::false_type());
             }
             total += (part[0].x + part[0].y) + (part[1].x + part[1].y);
         }

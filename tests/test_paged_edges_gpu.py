@@ -295,6 +295,16 @@ def check_beside_nan(dtype, nq, nkv, d, lens, new, bad, window=0, sinks=0):
         assert torch.equal(torch.isnan(out[rows]), nan[..., None].expand(-1, -1, d))
         close(lse[rows][~nan], z[~nan], zb[~nan], f"lse of sequence {b}")
         close(out[rows][~nan], o[~nan], ob[~nan], f"out of sequence {b}")
+        # the totals: of each token's weights where it sees a position
+        j = torch.arange(n, device=DEV)
+        seen = is_visible(t, j, window, sinks)
+        touched = (seen[:, None, :] & nan.view(m, nkv, -1).any(-1)[..., None]).any(0)
+        assert torch.equal(torch.isnan(mass[b, :, :n]), touched)
+        # positions that no NaN token sees: the other tokens' weights
+        clean = q[rows].clone()
+        clean[nan] = 0
+        _, _, _, _, w, wb = reference(c, b, clean, t, d ** -0.5, window, sinks)
+        close(mass[b, :, :n][~touched], w[~touched], wb[~touched], f"mass of sequence {b}")
 
 
 @pytest.mark.parametrize("dtype,nq,nkv,d", [(BF16, 8, 4, 256), (F16, 4, 2, 128), (BF16, 8, 1, 64), (F32, 4, 2, 64),
