@@ -41,7 +41,8 @@ __global__ void __launch_bounds__(128) paged_mass32_kernel(const PagedKv kv, con
 #pragma unroll
             for (int e = 0; e < E; ++e) d += k[e] * (qr[lane + 32 * e] * a.scale);
             d = warp_sum(d);
-            part += expf(d - a.lse[(first + i) * a.lse_row + head]);
+            const float z = a.lse[(first + i) * a.lse_row + head];
+            if (z != -INFINITY) part += expf(d - z);  // else the row has no weight at all
         }
         if ((i & 63) == 63) {
             sum += part;

@@ -353,3 +353,24 @@ def test_decode_queries_with_nan(dtype, nq, nkv, d):
         touched = torch.isnan(w)
         assert torch.equal(torch.isnan(mass[b, :, :n]), touched) and (mass[b, :, n:] == 0).all()
         close(mass[b, :, :n][~touched], w[~touched], wb[~touched], f"mass of sequence {b}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_scores_of_minus_infinity(dtype):
+    """Every visible score -inf: nothing carries weight, as with nothing visible."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([30, 40], 1, 64, 16, dtype)
+    q = queries(2, 2, 64, dtype, 0, False)
+    # over an f32 cache a product that overflows: an infinite element would have parts that are NaN
+    c.kp[c.table[0, :2].long(), 0, :, 0] = -2.0 ** 120 if dtype == F32 else -float("inf")
+    q[:1, :, 0] = 2.0 ** 120 if dtype == F32 else 1.0
+    mass = torch.zeros(2, 1, 40, device=DEV)
+    out, lse = paged.attend_decode(q, *c.args(), scale=0.1, mass=mass)
+    assert (out[0] == 0).all() and torch.isneginf(lse[0]).all() and (mass[0] == 0).all()
+    assert torch.isfinite(lse[1]).all() and abs(float(mass[1].sum()) - 2) < 1e-3
+    start = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    mass.zero_()
+    out, lse = paged.attend_prompt(q, start, 1, *c.args(), scale=0.1, mass=mass)
+    assert (out[0] == 0).all() and torch.isneginf(lse[0]).all() and (mass[0] == 0).all()
+    assert torch.isfinite(lse[1]).all() and abs(float(mass[1].sum()) - 2) < 1e-3
