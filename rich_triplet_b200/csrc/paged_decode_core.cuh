@@ -24,9 +24,10 @@
 // heads as its 8 columns (S^T = K Q^T, O^T = V^T P^T), so up to 8 heads read
 // each row at no extra cost; the memory stream leaves the tensor cores mostly
 // idle and tcgen05's 64-row operand would be mostly padding here.  The weights are split
-// in two 16-bit parts (hi + lo) before they multiply V, so their rounding
-// (2^-16) stays below the output's; with G <= 4 the low parts ride in columns
-// 4..7 of the same product.  f32 rows: tf32 products of hi and lo parts of
+// in two 16-bit parts (hi + lo) before they multiply V, so their rounding stays
+// below the output's: 2^-16 of a bf16 weight, 2^-22 of an f16 one, and where that
+// is less than f16's smallest step, 2^-32 of the largest weight (kLift).  With
+// G <= 4 the low parts ride in columns 4..7 of the same product.  f32 rows: tf32 products of hi and lo parts of
 // both operands, relative error about 2^-22; for the scores the queries are the
 // 16-row operand, hi parts above lo parts, so two products give all four terms.
 //
@@ -40,7 +41,7 @@
 // do not move the maximum, but their NaN is in the sum and in the output.
 //
 // The maximum is only moved when a score exceeds it by more than 8 (powers of
-// two), so weights stay below 2^8 and most tiles rescale nothing.
+// two), so weights stay below 2^8 (2^15 for f16 rows) and most tiles rescale nothing.
 #pragma once
 
 #include <math.h>
@@ -60,6 +61,10 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kSlotBytes = 8192;  // K or V rows of a tile, head_dim 256
 constexpr int kRingBytes = 3 * kSlotBytes;  // per warp
 constexpr float kMaxSlack = 8.f;
+// Weights of f16 rows are taken 2^7 above the largest one: f16's smallest step is
+// 2^-24, and with the slack of 2^8 they stay below its 65504.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
 constexpr int kMinFew = 4;
 
 template <typename T, int D, int NT>
@@ -424,7 +429,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
         }
 
         float o[NT][MT][4];
-        // of columns 2 t4 and 2 t4 + 1 (f32 rows: [0] of column g8); l: this lane's positions only
+        // of columns 2 t4 and 2 t4 + 1 (f32 rows: [0] of column g8); m: the weights are 2^(score - m),
+        // the maximum so far less kLift; l: this lane's positions only
         float m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -540,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                         seen = seen && p <= t && (a.window == 0 || p > t - a.window || p < a.sinks);
                     }
                     s[n][e] = seen ? s[n][e] : -INFINITY;
-                    over |= s[n][e] > m[n][q] + kMaxSlack;
+                    over |= s[n][e] > m[n][q] + (kMaxSlack + kLift<T>);
                 }
             if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -551,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_decode_kernel(const PagedKv
                         float v = F32 ? fmaxf(s[n][0], s[n][1]) : fmaxf(s[n][q], s[n][q + 2]);
 #pragma unroll
                         for (int d = F32 ? 1 : 4; d < (F32 ? 4 : 32); d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-                        const float mn = fmaxf(m[n][q], v);
+                        const float mn = fmaxf(m[n][q], v - kLift<T>);
                         f[q] = rel2(m[n][q], mn);
                         m[n][q] = mn;
                         l[n][q] *= f[q];

@@ -65,7 +65,15 @@ namespace {
 
 constexpr int kKeys = 128;   // positions of a key tile
 constexpr int kRows = 128;   // rows of a query tile
-constexpr float kMaxSlack = 8.f, kMaxWeight = 256.f;  // how far weights may exceed 1 (powers of two; their sum)
+// Weights are taken 2^kLift above the largest one, 7 for f16, whose smallest step
+// is 2^-24: a long tail of small weights then keeps its share (each is rounded by
+// at most 2^-32 of the largest).  kMaxSlack: how far they may exceed that before
+// the maximum is moved (powers of two; kMaxWeight: their sum), below f16's 65504.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
+constexpr float kMaxSlack = 8.f;
+template <typename T>
+constexpr float kMaxWeight = std::is_same<T, __half>::value ? 32768.f : 256.f;
 constexpr int kSoftRegs = 208, kOtherRegs = 88;
 constexpr int kMaxSplit = 16;  // CTAs that share a walk, at most
 
@@ -472,7 +480,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             const float2 sc = make_float2(wk.scale2, wk.scale2);
             float2 sum[2];
             uint32_t p[kKeys / 4];
-            float m2 = m == -INFINITY ? 0.f : m * wk.scale2;
+            float m2 = m == -INFINITY ? 0.f : m * wk.scale2 - kLift<T>;
             // The running maximum moves to the row's largest score so far.
             auto raise = [&]() {
                 float top[8];
@@ -486,7 +494,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                     for (int i = 0; i < q; ++i) top[i] = fmaxf(top[i], top[i + q]);
                 const float mn = fmaxf(m, top[0]), f = m == -INFINITY ? 0.f : tc::ex2((m - mn) * wk.scale2);
                 m = mn;
-                m2 = m == -INFINITY ? 0.f : m * wk.scale2;
+                m2 = m == -INFINITY ? 0.f : m * wk.scale2 - kLift<T>;
                 l *= f;
                 if (j == 0) return;
                 ok = tc::warp_wait(pv_done(t, j - 1), p_parity(j - 1), abort);
@@ -532,7 +540,7 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
                 weights(1);
                 const float s = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 const float t2 = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                return s > kMaxWeight || fmaf(t2, wk.scale2, -m2) > kMaxSlack;
+                return s > kMaxWeight<T> || fmaf(t2, wk.scale2, -m2) > kMaxSlack + kLift<T>;
             };
             const bool over = first_half();
             if (!fresh && __any_sync(0xffffffffu, over)) {
@@ -591,8 +599,8 @@ __global__ void __launch_bounds__(PCfg<D>::kThreads, 1)
             }
             if (live && ns == 1 && a.lse)
                 a.lse[(q_first + tok) * a.lse_row + head] =
-                    none ? -INFINITY : fmaf(m, wk.scale2, log2f(l)) * 0.693147180559945309f;
-            if (live && ns > 1) *reinterpret_cast<float2*>(rec + D) = make_float2(none ? -INFINITY : m * wk.scale2, l);
+                    none ? -INFINITY : fmaf(m, wk.scale2, log2f(l) - kLift<T>) * 0.693147180559945309f;
+            if (live && ns > 1) *reinterpret_cast<float2*>(rec + D) = make_float2(none ? -INFINITY : m * wk.scale2 - kLift<T>, l);
         }
         if (ns > 1) {
             // ---- the last of the walk's CTAs to get here joins their states in order ----

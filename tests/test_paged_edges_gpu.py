@@ -6,13 +6,14 @@ Tolerances are those derived in test_paged_gpu.py, whose caches and 64-bit
 definition are used here, except where a test says otherwise.
 """
 
+import math
 import threading
 
 import pytest
 import torch
 
 from rich_triplet_b200._lib import RtError
-from test_paged_gpu import BF16, DEV, F16, F32, Cache, close, is_visible, queries, reference
+from test_paged_gpu import BF16, DEV, F16, F32, Cache, close, e32, is_visible, queries, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -374,3 +375,58 @@ def test_scores_of_minus_infinity(dtype):
     out, lse = paged.attend_prompt(q, start, 1, *c.args(), scale=0.1, mass=mass)
     assert (out[0] == 0).all() and torch.isneginf(lse[0]).all() and (mass[0] == 0).all()
     assert torch.isfinite(lse[1]).all() and abs(float(mass[1].sum()) - 2) < 1e-3
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(4, 1, 64), (8, 1, 128), (12, 1, 256), (2, 1, 256)])
+@pytest.mark.parametrize("below", [20.0, 24.6, 25.3])
+@pytest.mark.parametrize("at", [0, -1])
+def test_f16_weights_far_below_the_largest(nq, nkv, d, below, at):
+    """One position 2^below heavier than each of 131070 others, which hold the
+    only values that are not 0: their share of the output must not be lost.
+
+    Weights are taken 2^7 above the largest one, so f16's smallest step rounds
+    each by at most 2^-25 2^-7, and all of them by n 2^-32 of the sum, which is at
+    least the largest weight; the rest of the bound is that of every output."""
+    from rich_triplet_b200 import paged
+
+    n, page = 131071, 256
+    scale = d ** -0.5
+    c = Cache.__new__(Cache)
+    c.lens, c.page, c.dtype, c.nkv, c.d = [n], page, F16, nkv, d
+    k = torch.zeros(nkv, n, d, dtype=F16, device=DEV)
+    v = torch.ones(nkv, n, d, dtype=F16, device=DEV)
+    k[:, at, 0], v[:, at] = 8.0, 0.0
+    c.k, c.v = [k.double()], [v.double()]
+    pages = -(-n // page)
+    kp, vp = (torch.nn.functional.pad(x, (0, 0, 0, pages * page - n)).view(nkv, pages, page, d).transpose(0, 1).contiguous()
+              for x in (k, v))
+    table = torch.arange(pages, dtype=torch.int32, device=DEV).view(1, -1)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    q = torch.zeros(3, nq, d, dtype=F16, device=DEV)
+    q[:, :, 0] = below * math.log(2.0) / 8.0 / scale
+    u, e = 2.0 ** -11, e32(n)
+
+    def check(out, lse, t, what):
+        o, _, z, zb, _, _ = reference(c, 0, q[:len(t)], t, scale, 0, 0)
+        delta = 2 * e32(d) * below  # the one product's size
+        A = o.abs()
+        bound = u * (o.abs() + A) + (2 * delta + 2 * e) * A + n * 2.0 ** -32 + 2.0 ** -25
+        close(out, o.expand_as(out), bound.expand_as(out), what)
+        close(lse, z.expand_as(lse), zb.expand_as(lse), what + " lse")
+        assert float((o - bound).min()) > 0  # nothing would not do
+
+    out, lse = paged.attend_decode(q[:1], kp, vp, table, lens, scale=scale)
+    check(out, lse, torch.tensor([n - 1], device=DEV), "decode")
+    # sequences on the same pages, so many that hardly one is split over CTAs
+    many = 300
+    shared = (kp, vp, table.expand(many, -1), lens.repeat(many))
+    qs = q[:1].expand(many, -1, -1)
+    out, lse = paged.attend_decode(qs, *shared, scale=scale)
+    check(out, lse, torch.tensor([n - 1], device=DEV), "decode of many")
+    start = torch.arange(many + 1, dtype=torch.int32, device=DEV)
+    out, lse = paged.attend_prompt(qs, start, 1, *shared, scale=scale)
+    check(out, lse, torch.tensor([n - 1], device=DEV), "prompt of many")
+    if at == 0:  # every token sees the heavy position
+        start = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+        out, lse = paged.attend_prompt(q, start, 3, kp, vp, table, lens, scale=scale)
+        check(out, lse, torch.arange(n - 3, n, device=DEV), "prompt")
