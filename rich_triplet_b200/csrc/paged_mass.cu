@@ -273,9 +273,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         };
         // rows of the tokens that see position j: [see, until)
-        const int see = max(0, (j - pos0) * G);
+        // (counts of tokens are cut to those of the call before they are multiplied: positions times G pass 32 bits)
+        const int see = min(max(0, j - pos0), i_hi + 1) * G;
         const int until = a.window > 0 && j >= a.sinks
-                              ? static_cast<int>(min(static_cast<int64_t>(r_end), (static_cast<int64_t>(j) + a.window - pos0) * G)) : r_end;
+                              ? static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(i_hi) + 1, static_cast<int64_t>(j) + a.window - pos0))) * G
+                              : r_end;
         load_rows(grp);
         bool ok = true;
         for (int i = grp; i < n; i += kSumGroups) {

@@ -430,3 +430,42 @@ def test_f16_weights_far_below_the_largest(nq, nkv, d, below, at):
         start = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
         out, lse = paged.attend_prompt(q, start, 3, kp, vp, table, lens, scale=scale)
         check(out, lse, torch.arange(n - 3, n, device=DEV), "prompt")
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1000, 200)])
+def test_totals_of_more_positions_than_32_bits_hold_rows(window, sinks):
+    """2^27 and some positions times 16 heads pass 2^31 (all on one page of 256
+    rows, so the weights of a slot are equal everywhere)."""
+    from rich_triplet_b200 import paged
+
+    n, page, d, G = 2 ** 27 + 2 ** 12, 256, 64, 16
+    g = torch.Generator().manual_seed(1)
+    kp, vp = (torch.randn(1, 1, page, d, generator=g).to(DEV).to(BF16) for _ in range(2))
+    table = torch.zeros(1, n // page, dtype=torch.int32, device=DEV)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    q = queries(2, G, d, BF16, 0, False)
+    start = torch.tensor([0, 2], dtype=torch.int32, device=DEV)
+    mass = torch.zeros(1, 1, n, device=DEV)
+    paged.attend_prompt(q, start, 2, kp, vp, table, lens, scale=0.125, window=window, sinks=sinks, mass=mass)
+    s = torch.exp(torch.einsum("tgd,pd->tgp", q.double(), kp[0, 0].double()) * 0.125)  # of a slot
+    want = torch.zeros(n, dtype=torch.float64, device=DEV)
+    for i in range(2):
+        t = n - 2 + i
+        count = torch.zeros(n, dtype=torch.bool, device=DEV)
+        if window:
+            count[:sinks] = True
+            count[t + 1 - window:t + 1] = True
+        else:
+            count[:t + 1] = True
+        seen = count.view(-1, page)
+        total = (seen.sum(0).double()[None] * s[i]).sum(1, keepdim=True)
+        want += (seen * (s[i] / total).sum(0)).flatten()
+    got = mass[0, 0].double()
+    same = bool(((got > 0) == (want > 0)).all())
+    assert same
+    # relative: a score's error, 2 e32(d) of at most 64 x 5 x 5 x 0.125, and 2^16 additions to a row's sum
+    worst = float(((got - want).abs() - want * 1e-2).max())
+    assert worst <= 0
+    assert abs(float(got.sum()) - 2 * G) < 0.1
+    del mass, got, want
+    torch.cuda.empty_cache()
