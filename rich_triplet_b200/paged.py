@@ -188,6 +188,8 @@ class PagedKvCache:
     def extend(self, counts):
         """Room for counts[b] new tokens of every sequence b: lengths grow and
         pages are taken from the pool."""
+        if any(c < 0 for c in counts):
+            raise ValueError(f"PagedKvCache.extend: negative counts {list(counts)}")
         wanted = [n + c for n, c in zip(self.lens, counts)]
         if len(counts) != len(self.lens) or max(wanted) > self.max_len:
             raise ValueError(f"PagedKvCache.extend: lengths {wanted} for {len(self.lens)} sequences of at most "

@@ -7,7 +7,7 @@ import subprocess
 import sys
 
 import pytest
-import torch  # noqa: F401
+import torch
 
 
 def test_forget_and_sync_without_a_context():
@@ -70,3 +70,26 @@ def test_scratch_of_any_sizes_answers():
     # 3 x 4 rows of 5 pages of 16 positions, and their maxima and sums
     assert got[0] == (0, 256 + 3840)
     assert [status for status, _ in got[1:]] == [-4] * len(bad)
+
+
+def cache(layers=2, sequences=3, pages=12, page=8, heads=1, d=64, max_len=64, **kw):
+    from rich_triplet_b200.paged import PagedKvCache
+
+    return PagedKvCache(layers, sequences, pages, page, heads, d, max_len, device="cpu", **kw)
+
+
+def accounted(c):
+    """Every page is in the table once or free once."""
+    used = [int(p) for p in c.page_table.flatten() if p >= 0]
+    assert torch.equal(c.page_table, c._table) and c.lens_device.tolist() == c.lens
+    return sorted(used + c.pool._free) == list(range(c.pool.num_pages))
+
+
+def test_extend_refuses_negative_counts():
+    c = cache()
+    c.extend([9, 1, 16])
+    with pytest.raises(ValueError, match="negative counts"):
+        c.extend([-9, 0, 0])
+    assert c.lens == [9, 1, 16] and accounted(c)
+    c.extend([7, 7, 1])
+    assert c.lens == [16, 8, 17] and accounted(c)
