@@ -232,14 +232,21 @@ class PagedKvCache:
         positions of each layer."""
         if self.mass is None:
             raise ValueError("PagedKvCache.evict: the cache was made without totals")
+        if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+            raise ValueError(f"PagedKvCache.evict: sinks {sinks} + recent {recent} must lie in 0..budget {budget}")
         each = -(-budget // self.page_size)
-        dst = torch.tensor(self.pool.take(each * len(self.lens)), dtype=torch.int32).view(len(self.lens), each)
-        on_device = dst.to(self.device)
-        kept = []
-        for i in range(self.k.shape[0]):
-            got, _, self.mass[i] = kv_evict(self.k[i], self.v[i], self.page_table, self.lens_device, self.mass[i],
-                                            on_device, budget=budget, sinks=sinks, recent=recent)
-            kept.append(got)
+        pages = self.pool.take(each * len(self.lens))
+        try:
+            dst = torch.tensor(pages, dtype=torch.int32).view(len(self.lens), each)
+            on_device = dst.to(self.device)
+            done = [kv_evict(self.k[i], self.v[i], self.page_table, self.lens_device, self.mass[i], on_device,
+                             budget=budget, sinks=sinks, recent=recent) for i in range(self.k.shape[0])]
+        except Exception:
+            self.pool.give(pages)  # the sequences still have theirs
+            raise
+        kept = [got for got, _, _ in done]
+        for i, (_, _, mass) in enumerate(done):
+            self.mass[i] = mass
         self.pool.give([int(p) for p in self._table.flatten() if p >= 0])
         self.lens = [min(n, budget) for n in self.lens]
         self._table.fill_(-1)

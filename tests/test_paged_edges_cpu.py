@@ -93,3 +93,86 @@ def test_extend_refuses_negative_counts():
     assert c.lens == [9, 1, 16] and accounted(c)
     c.extend([7, 7, 1])
     assert c.lens == [16, 8, 17] and accounted(c)
+
+
+def plain_evict(k, v, table, lens, mass, dst, *, budget, sinks=0, recent=0):
+    """kv_evict in plain torch."""
+    page = k.shape[2]
+    kept = torch.full((len(lens), k.shape[1], budget), -1, dtype=torch.int32)
+    out = torch.zeros_like(mass)
+    for b, n in enumerate(lens.tolist()):
+        for h in range(k.shape[1]):
+            ends = [j for j in range(n) if j < sinks or j >= n - recent] if n > budget else range(n)
+            rest = sorted(set(range(n)) - set(ends), key=lambda j: (-float(mass[b, h, j]), j))
+            keep = sorted((list(ends) + rest)[:budget])
+            for i, j in enumerate(keep):
+                kept[b, h, i], out[b, h, i] = j, mass[b, h, j]
+                for pool in (k, v):
+                    pool[dst[b, i // page], h, i % page] = pool[table[b, j // page], h, j % page]
+    return kept, lens.clamp(max=budget), out
+
+
+def filled(monkeypatch, lens, **kw):
+    from rich_triplet_b200 import paged
+
+    monkeypatch.setattr(paged, "kv_evict", plain_evict)
+    c = cache(sequences=len(lens), totals=True, **kw)
+    c.extend(lens)
+    g = torch.Generator().manual_seed(2)
+    for b, n in enumerate(lens):
+        c.mass[:, b, :, :n] = torch.rand(c.mass.shape[0], c.mass.shape[2], n, generator=g)
+        for j in range(n):
+            at = int(c.page_table[b, j // c.page_size]), slice(None), j % c.page_size
+            for layer in range(c.k.shape[0]):
+                c.k[layer][at] = 1000.0 * layer + 100 * b + j
+                c.v[layer][at] = -(1000.0 * layer + 100 * b + j)
+    return c
+
+
+def check_trimmed(c, lens, before, kept, budget, sinks, recent):
+    """The cache holds what a trim of `lens` positions with totals `before` leaves."""
+    assert c.lens == [min(n, budget) for n in lens] and accounted(c)
+    for layer in range(c.k.shape[0]):
+        for b, n in enumerate(lens):
+            m = min(n, budget)
+            for h in range(c.k.shape[2]):
+                ends = [j for j in range(n) if j < sinks or j >= n - recent] if n > budget else range(n)
+                rest = sorted(set(range(n)) - set(ends), key=lambda j: (-float(before[layer, b, h, j]), j))
+                keep = sorted((list(ends) + rest)[:budget])
+                assert kept[layer][b, h].tolist() == keep + [-1] * (budget - m)
+                assert c.mass[layer, b, h, :m].tolist() == [float(before[layer, b, h, j]) for j in keep]
+                assert (c.mass[layer, b, h, m:] == 0).all()
+                for i, j in enumerate(keep):
+                    at = int(c.page_table[b, i // c.page_size]), h, i % c.page_size
+                    assert (c.k[layer][at] == 1000.0 * layer + 100 * b + j).all()
+                    assert (c.v[layer][at] == -(1000.0 * layer + 100 * b + j)).all()
+
+
+def test_evict(monkeypatch):
+    lens = [40, 7, 0, 16, 33]
+    c = filled(monkeypatch, lens, pages=32, heads=2, dtype=torch.float32)
+    before = c.mass.clone()
+    check_trimmed(c, lens, before, c.evict(16, sinks=2, recent=5), 16, 2, 5)
+
+
+def test_evict_that_is_refused_changes_nothing(monkeypatch):
+    from rich_triplet_b200 import paged
+
+    lens = [40, 7]
+    c = filled(monkeypatch, lens, pages=20, dtype=torch.float32)
+    mass, table = c.mass.clone(), c.page_table.clone()
+    for kw in (dict(budget=16, sinks=10, recent=7), dict(budget=0), dict(budget=16, sinks=-1), dict(budget=16, recent=-1)):
+        with pytest.raises(ValueError, match="must lie in"):
+            c.evict(**kw)
+    calls = []
+
+    def fails_late(*a, **kw):
+        calls.append(1)
+        if len(calls) == 2:
+            raise RuntimeError("a launch failed")
+        return plain_evict(*a, **kw)
+
+    monkeypatch.setattr(paged, "kv_evict", fails_late)
+    with pytest.raises(RuntimeError, match="a launch failed"):
+        c.evict(16)
+    assert c.lens == lens and accounted(c) and torch.equal(c.mass, mass) and torch.equal(c.page_table, table)
