@@ -227,32 +227,65 @@ class PagedKvCache:
                              scale=scale, window=window, sinks=sinks, mass=mass)
 
     def evict(self, budget, sinks=0, recent=0):
-        """Trim every sequence of every layer to ``budget`` positions by its
-        totals (kv_evict); the old pages go back to the pool.  Returns the kept
-        positions of each layer."""
+        """Trim every sequence of every layer that is longer than ``budget``
+        positions to so many by its totals (kv_evict); its old pages go back to the
+        pool.  Returns the kept positions of each layer.  Sequences take turns
+        where the pool has too few free pages for all of them; with none to spare
+        one is trimmed through a copy of its rows outside the pool."""
         if self.mass is None:
             raise ValueError("PagedKvCache.evict: the cache was made without totals")
         if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
             raise ValueError(f"PagedKvCache.evict: sinks {sinks} + recent {recent} must lie in 0..budget {budget}")
+        layers, _, heads = self.mass.shape[:3]
         each = -(-budget // self.page_size)
-        pages = self.pool.take(each * len(self.lens))
+        at = torch.arange(budget, dtype=torch.int32, device=self.device)
+        kept = torch.where(at < self.lens_device[:, None, None], at, -1).repeat(layers, 1, heads, 1)
+        left = [b for b, n in enumerate(self.lens) if n > budget]
+        while left:
+            now = max(1, self.pool.free_pages // each)
+            self._trim(left[:now], kept, each, dict(budget=budget, sinks=sinks, recent=recent))
+            left = left[now:]
+        return list(kept)
+
+    def _trim(self, seqs, kept, each, limits):
+        """Trims sequences `seqs` into `each` pages each: free ones, or, for one
+        sequence, as many of its own as are wanting."""
+        own = [[int(p) for p in self._table[b] if p >= 0] for b in seqs]
+        short = max(0, each * len(seqs) - self.pool.free_pages)
+        if short > (len(own[0]) if len(seqs) == 1 else 0):
+            raise ValueError(f"PagedKvCache.evict: {short} more pages wanted than are free")
+        taken = self.pool.take(each * len(seqs) - short)
         try:
-            dst = torch.tensor(pages, dtype=torch.int32).view(len(self.lens), each)
-            on_device = dst.to(self.device)
-            done = [kv_evict(self.k[i], self.v[i], self.page_table, self.lens_device, self.mass[i], on_device,
-                             budget=budget, sinks=sinks, recent=recent) for i in range(self.k.shape[0])]
+            pages = torch.tensor(taken + own[0][:short], dtype=torch.int32).view(len(seqs), each)
+            dst = pages.to(self.device)
+            rows = slice(None) if len(seqs) == len(self.lens) else torch.tensor(seqs, device=self.device)
+            lens = self.lens_device[rows]
+            if short:  # the sequence's pages and `each` more, in pools of their own
+                at = torch.tensor(own[0], device=self.device)
+                table = torch.full_like(self._table[seqs], -1)
+                table[self._table[seqs] >= 0] = torch.arange(len(own[0]), dtype=torch.int32)
+                table = table.to(self.device)
+                spare = torch.arange(len(own[0]), len(own[0]) + each, dtype=torch.int32, device=self.device).view(1, -1)
+            done = []
+            for k, v, mass in zip(self.k, self.v, self.mass):
+                if not short:
+                    done.append(kv_evict(k, v, self.page_table[rows], lens, mass[rows], dst, **limits))
+                else:
+                    room = [torch.cat([x[at], x.new_zeros((each, *x.shape[1:]))]) for x in (k, v)]
+                    done.append((*kv_evict(*room, table, lens, mass[rows], spare, **limits),
+                                 *(x[len(own[0]):] for x in room)))
         except Exception:
-            self.pool.give(pages)  # the sequences still have theirs
+            self.pool.give(taken)  # the sequences still have theirs
             raise
-        kept = [got for got, _, _ in done]
-        for i, (_, _, mass) in enumerate(done):
-            self.mass[i] = mass
-        self.pool.give([int(p) for p in self._table.flatten() if p >= 0])
-        self.lens = [min(n, budget) for n in self.lens]
-        self._table.fill_(-1)
-        for b, n in enumerate(self.lens):
-            used = -(-n // self.page_size)
-            self._table[b, :used] = dst[b, :used]
-            self.pool.give(dst[b, used:].tolist())
+        for i, (got, _, mass, *moved) in enumerate(done):
+            kept[i, rows] = got
+            self.mass[i, rows] = mass
+            for x, rest in zip((self.k, self.v), moved):
+                x[i, dst[0].long()] = rest
+        kept_own = own[0][:short]
+        self.pool.give([p for ids in own for p in ids if p not in kept_own])
+        for b, ids in zip(seqs, pages):
+            self.lens[b] = limits["budget"]
+            self._table[b] = -1
+            self._table[b, :each] = ids
         self._upload()
-        return kept

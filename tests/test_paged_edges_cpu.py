@@ -176,3 +176,33 @@ def test_evict_that_is_refused_changes_nothing(monkeypatch):
     with pytest.raises(RuntimeError, match="a launch failed"):
         c.evict(16)
     assert c.lens == lens and accounted(c) and torch.equal(c.mass, mass) and torch.equal(c.page_table, table)
+
+
+@pytest.mark.parametrize("spare", [0, 1, 2, 5, 30])
+def test_evict_in_a_pool_with_few_free_pages(monkeypatch, spare):
+    """Sequences take turns on the free pages; with none, one at a time goes
+    through a copy outside the pool.  Those within the budget keep their pages."""
+    lens = [40, 7, 0, 17, 33, 64]
+    used = sum(-(-n // 8) for n in lens)
+    c = filled(monkeypatch, lens, pages=used + spare, heads=2, dtype=torch.float32)
+    before, short = c.mass.clone(), c.page_table[1].clone()
+    assert c.pool.free_pages == spare
+    check_trimmed(c, lens, before, c.evict(16, sinks=2, recent=5), 16, 2, 5)
+    assert torch.equal(c.page_table[1], short)
+    # 16 positions in 2 pages each now, but for 7 in one and none
+    assert c.pool.num_pages - c.pool.free_pages == 9
+
+
+def test_evict_after_dropped_pages(monkeypatch):
+    """Dropped positions have no rows to keep: their slots read as zeros, and the
+    page counts still add up, in a full pool too."""
+    c = filled(monkeypatch, [64, 40], pages=13, dtype=torch.float32)
+    c.drop(window=20)
+    assert accounted(c)
+    c.pool.take(c.pool.free_pages)  # someone else has the rest
+    monkeypatch.setattr("rich_triplet_b200.paged.kv_evict", lambda k, v, table, lens, mass, dst, *, budget, **kw: (
+        torch.zeros(len(lens), 1, budget, dtype=torch.int32), lens.clamp(max=budget), torch.zeros_like(mass)))
+    c.evict(16)
+    assert c.lens == [16, 16]
+    used = [int(p) for p in c.page_table.flatten() if p >= 0]
+    assert len(set(used)) == 4 and torch.equal(c.page_table, c._table)

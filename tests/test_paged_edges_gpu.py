@@ -469,3 +469,36 @@ def test_totals_of_more_positions_than_32_bits_hold_rows(window, sinks):
     assert abs(float(got.sum()) - 2 * G) < 0.1
     del mass, got, want
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("spare", [0, 3, 60])
+def test_cache_trims_in_full_pools(spare):
+    """PagedKvCache.evict with none, a few and enough free pages: the rows and
+    totals of kv_evict."""
+    from rich_triplet_b200 import paged
+
+    lens, page, d = [700, 90, 0, 301, 1000], 16, 64
+    used = sum(-(-n // page) for n in lens)
+    c = paged.PagedKvCache(2, 5, used + spare, page, 2, d, 1024, BF16, totals=True)
+    c.extend(lens)
+    k = torch.randn(2, c.pool.num_pages, 2, page, d, device=DEV).to(BF16)
+    c.k.copy_(k)
+    c.v.copy_(-k)
+    live = torch.arange(1024, device=DEV) < c.lens_device[:, None, None]
+    c.mass.copy_(torch.rand(2, 5, 2, 1024, device=DEV) * live)
+    want = []
+    for i in range(2):  # all five, into pages behind the pool's
+        room = [torch.cat([x[i], torch.zeros(5 * 8, 2, page, d, dtype=BF16, device=DEV)]) for x in (c.k, c.v)]
+        dst = torch.arange(c.pool.num_pages, c.pool.num_pages + 40, dtype=torch.int32, device=DEV).view(5, 8)
+        want.append((*paged.kv_evict(*room, c.page_table, c.lens_device, c.mass[i], dst, budget=120, sinks=4, recent=30),
+                     room, dst))
+    kept = c.evict(120, sinks=4, recent=30)
+    assert c.lens == [120, 90, 0, 120, 120]
+    for i, (positions, lens_t, mass, room, dst) in enumerate(want):
+        assert torch.equal(kept[i], positions) and torch.equal(c.lens_device, lens_t) and torch.equal(c.mass[i], mass)
+        for b, n in enumerate(c.lens):
+            j = torch.arange(n, device=DEV)
+            for x, y in zip((c.k[i], c.v[i]), room):
+                assert torch.equal(x[c.page_table[b, j // page].long(), :, j % page], y[dst[b, j // page].long(), :, j % page])
+    used = [int(p) for p in c.page_table.flatten() if p >= 0]
+    assert sorted(used + c.pool._free) == list(range(c.pool.num_pages))
