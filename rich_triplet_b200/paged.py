@@ -204,7 +204,12 @@ class PagedKvCache:
 
     def drop(self, window, sinks=0):
         """Give back the pages that no later token sees: before the window of
-        the next one, and past the first ``sinks`` positions."""
+        the next one, and past the first ``sinks`` positions (none with a window
+        of 0, which sees everything)."""
+        if window < 0 or sinks < 0:
+            raise ValueError(f"PagedKvCache.drop: negative window {window} or sinks {sinks}")
+        if window == 0:
+            return
         first = -(-sinks // self.page_size)
         for b, n in enumerate(self.lens):
             for p in range(first, max(0, n + 1 - window) // self.page_size):

@@ -206,3 +206,33 @@ def test_evict_after_dropped_pages(monkeypatch):
     assert c.lens == [16, 16]
     used = [int(p) for p in c.page_table.flatten() if p >= 0]
     assert len(set(used)) == 4 and torch.equal(c.page_table, c._table)
+
+
+def test_drop_takes_back_what_no_later_token_sees():
+    """Any order of growth, windows and first tokens: the pages that one pass over
+    every table entry would give back, once each."""
+    import random
+
+    rng = random.Random(3)
+    for _ in range(60):
+        c = cache(layers=1, sequences=3, pages=30, max_len=80)
+        table = [[-1] * 10 for _ in range(3)]  # which entries hold a page
+        for _ in range(25):
+            if rng.random() < 0.6:
+                counts = [rng.randint(0, min(9, 80 - n)) for n in c.lens]
+                for b, (n, m) in enumerate(zip(c.lens, counts)):
+                    for p in range(-(-n // 8), -(-(n + m) // 8)):
+                        table[b][p] = 1
+                c.extend(counts)
+            else:
+                window, sinks = rng.choice([0, 1, 5, 8, 20, 33, 70]), rng.choice([0, 0, 1, 8, 9, 30])
+                if window:
+                    for b, n in enumerate(c.lens):
+                        for p in range(-(-sinks // 8), max(0, n + 1 - window) // 8):
+                            table[b][p] = -1
+                c.drop(window, sinks)
+            assert [[min(1, max(-1, int(x))) if x < 0 else 1 for x in row] for row in c.page_table] == table
+            assert accounted(c)
+    for bad in ((-1, 0), (4, -1)):
+        with pytest.raises(ValueError, match="negative"):
+            c.drop(*bad)
