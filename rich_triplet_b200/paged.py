@@ -173,6 +173,7 @@ class PagedKvCache:
         self.page_size, self.max_len, self.device = page_size, max_len, self.k.device
         self.pool = PagePool(num_pages)
         self.lens = [0] * sequences
+        self._gone = [(0, 0)] * sequences  # table entries [from, to) whose pages drop() gave back
         width = -(-max_len // page_size)
         self._table = torch.full((sequences, width), -1, dtype=torch.int32)
         self.page_table = self._table.to(self.device)
@@ -181,8 +182,9 @@ class PagedKvCache:
         if totals:
             self.mass = torch.zeros((layers, sequences, kv_heads, max_len), dtype=torch.float32, device=self.device)
 
-    def _upload(self):
-        self.page_table.copy_(self._table)
+    def _upload(self, table=True):
+        if table:
+            self.page_table.copy_(self._table)
         self.lens_device.copy_(torch.tensor(self.lens, dtype=torch.int32))
 
     def extend(self, counts):
@@ -200,7 +202,7 @@ class PagedKvCache:
             for p in r:
                 self._table[b, p] = pages.pop()
         self.lens = wanted
-        self._upload()
+        self._upload(table=any(need))
 
     def drop(self, window, sinks=0):
         """Give back the pages that no later token sees: before the window of
@@ -210,13 +212,20 @@ class PagedKvCache:
             raise ValueError(f"PagedKvCache.drop: negative window {window} or sinks {sinks}")
         if window == 0:
             return
-        first = -(-sinks // self.page_size)
+        first, given = -(-sinks // self.page_size), []
         for b, n in enumerate(self.lens):
-            for p in range(first, max(0, n + 1 - window) // self.page_size):
-                if self._table[b, p] >= 0:
-                    self.pool.give([int(self._table[b, p])])
+            end = max(0, n + 1 - window) // self.page_size
+            lo, hi = self._gone[b]
+            for p in (*range(first, min(lo, end)), *range(max(hi, first), end)):
+                page = int(self._table[b, p])
+                if page >= 0:
+                    given.append(page)
                     self._table[b, p] = -1
-        self._upload()
+            if first < end and (lo == hi or first <= hi and lo <= end):  # else two gaps: the older one is remembered
+                self._gone[b] = (first, end) if lo == hi else (min(lo, first), max(hi, end))
+        if given:
+            self.pool.give(given)
+            self.page_table.copy_(self._table)
 
     def append(self, layer, k, v, q_start=None):
         kv_append(self.k[layer], self.v[layer], k, v, self.page_table, self.lens_device, q_start)
@@ -293,4 +302,5 @@ class PagedKvCache:
             self.lens[b] = limits["budget"]
             self._table[b] = -1
             self._table[b, :each] = ids
+            self._gone[b] = (0, 0)
         self._upload()

@@ -236,3 +236,22 @@ def test_drop_takes_back_what_no_later_token_sees():
     for bad in ((-1, 0), (4, -1)):
         with pytest.raises(ValueError, match="negative"):
             c.drop(*bad)
+
+
+def test_drop_every_step_costs_the_same_late_in_a_long_sequence():
+    """A step's drop looks at the entries that it gives back, not at all of them."""
+    seen = []
+
+    class Watched(torch.Tensor):
+        def __getitem__(self, at):
+            seen.append(at)
+            return super().__getitem__(at)
+
+    c = cache(layers=1, sequences=8, pages=8 * 4200, max_len=32768)
+    c.extend([32000] * 8)
+    c.drop(1024, 4)
+    c._table = c._table.as_subclass(Watched)
+    for _ in range(32):
+        c.extend([1] * 8)
+        c.drop(1024, 4)
+    assert len(seen) <= 2 * 8 * 32 // 8 + 8 and accounted(c)
