@@ -51,6 +51,10 @@ class _DeviceContext(Context):
         """Waits for all streams of the device and raises RtError if a kernel
         reported that a bounded wait gave up since the last sync()."""
         torch.cuda.synchronize(self.device)
+        self.check()
+
+    def check(self):
+        """The same for kernels that have finished, without waiting for streams."""
         _ext.sync(self.device)
 
     def close(self):

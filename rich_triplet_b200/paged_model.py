@@ -19,6 +19,7 @@ import time
 import numpy as np
 import torch
 
+from . import paged
 from .model import Config4, Gemma3Weights, MatBf16, Q4KMat, synth_gemma3, synth_tokens
 from .ops import Context
 from .paged import PagedKvCache
@@ -94,6 +95,13 @@ class PagedGemma3:
         logits.record_stream(caller)
         return logits
 
+    def sync(self):
+        """Waits for the steps so far; raises RtError if one of their kernels
+        reported that a bounded wait gave up (as the next step would)."""
+        self.stream.synchronize()
+        self.ctx.sync()
+        paged.context(self.stream.device).check()
+
     def _step(self, tokens):
         cfg, D = self.cfg, self.cfg.head_dim
         nq, nkv = cfg.num_attention_heads, cfg.num_key_value_heads
@@ -110,6 +118,8 @@ class PagedGemma3:
         q_start = None if decode else torch.tensor(starts, dtype=torch.int32).cuda()
         ids = torch.tensor(flat).cuda()
         at = torch.tensor(np.concatenate([np.arange(p, p + c) for p, c in zip(self.position, counts)])).cuda()
+        # those copies waited for the last step: its kernels' reports are there
+        paged.context(self.stream.device).check()
         for c in self.caches:
             if c is not None:
                 c.extend(counts)
@@ -166,14 +176,14 @@ def main(argv=None):
     torch.cuda.synchronize()
     t0 = time.perf_counter()
     logits = model.step(prompts)
-    torch.cuda.synchronize()
+    model.sync()
     t1 = time.perf_counter()
     for _ in range(a.steps):
         tok = logits.argmax(-1).tolist()
         for o, t in zip(out, tok):
             o.append(t)
         logits = model.step([[t] for t in tok])
-    torch.cuda.synchronize()
+    model.sync()
     t2 = time.perf_counter()
     kept = "no global layer" if model.caches[1] is None else f"global layers hold {model.caches[1].lens}"
     print(f"paged_model: {a.seqs} sequences, {a.layers} layers, prompts {[len(p) for p in prompts]}: prompt step "

@@ -67,3 +67,34 @@ def test_tokens_and_positions_out_of_range_are_refused(tiny):
     assert torch.equal(model.step(tok), other.step(tok))
     model.step([[1] * 12, [1]])  # up to the last position
     assert model.position == [16, 3]
+
+
+def test_a_wait_that_gave_up_is_reported(tiny, monkeypatch):
+    """The attention kernels report to the paged operators' context: the next step
+    and sync() ask it (here a stand-in for its error word)."""
+    from rich_triplet_b200 import paged
+    from rich_triplet_b200._lib import RT_E_TIMEOUT, RtError
+    from rich_triplet_b200.paged_model import PagedGemma3
+
+    cfg, w = tiny
+    model = PagedGemma3(w, 1, 16, page_size=8, dtype=torch.float16)
+    model.step([[1, 2, 3]])
+    model.sync()
+    asked = []
+
+    def gave_up(self):
+        asked.append(self)
+        raise RtError(RT_E_TIMEOUT, "a kernel reported error word 1 (bounded wait gave up)")
+
+    with monkeypatch.context() as m:
+        m.setattr(paged._DeviceContext, "check", gave_up)
+        with pytest.raises(RtError, match="gave up"):
+            model.step([[4]])
+        with pytest.raises(RtError, match="gave up"):
+            model.sync()
+        with pytest.raises(RtError, match="gave up"):
+            paged.context("cuda").sync()
+    assert asked == [paged.context("cuda")] * 3
+    assert model.position == [3] and model.caches[0].lens == [3]  # refused before the step
+    model.step([[4]])
+    model.sync()
