@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -66,6 +67,14 @@ const at::Tensor* tensor(PyObject* o, const char* name) {
     return &THPVariable_Unpack(o);
 }
 
+// Nothing here is differentiable: inputs that want gradients are refused, where
+// gradients are recorded, instead of being cut out of them silently.
+template <typename... T>
+bool no_gradients(const char* who, const T*... t) {
+    if (!at::GradMode::is_enabled() || !((t && t->requires_grad()) || ...)) return true;
+    return value_error("%s is not differentiable: call it under torch.no_grad()", who);
+}
+
 // The stream that torch uses now on the device.  The default stream's handle is
 // null, which the library takes for the context's own: it is named by CUDA's
 // value for it.
@@ -89,6 +98,7 @@ bool int32_rows(const at::Tensor& t, int index, int64_t n) {
 
 struct Cache {
     rt_paged_kv kv;
+    const at::Tensor *k, *v;
     at::ScalarType type;
     int index;
 };
@@ -113,6 +123,8 @@ bool get_cache(PyObject* const* a, Cache* c) {
     if (!int32_rows(*lens, c->index, n)) return value_error("paged: lens must be [%lld] int32, contiguous, on the pools' GPU", n);
     if (n > INT32_MAX || width > INT32_MAX || k->size(1) > INT32_MAX || k->size(2) > INT32_MAX || k->size(3) > INT32_MAX)
         return value_error("paged: a size does not fit 32 bits");
+    c->k = k;
+    c->v = v;
     rt_paged_kv& kv = c->kv;
     kv.k = k->data_ptr();
     kv.v = v->data_ptr();
@@ -157,7 +169,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Cache c;
         if (!get_cache(a, &c)) return nullptr;
         const at::Tensor *k = tensor(a[4], "k"), *v = tensor(a[5], "v");
-        if (!k || !v) return nullptr;
+        if (!k || !v || !no_gradients("kv_append", k, v, c.k, c.v)) return nullptr;
         if (k->dim() != 3 || v->sizes() != k->sizes() || v->strides() != k->strides() || k->size(1) != c.kv.kv_heads ||
             k->size(2) != c.kv.head_dim || k->stride(2) != 1) {
             value_error("kv_append: k and v must be [rows, %d, %d] with the same strides and contiguous rows",
@@ -227,6 +239,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
             }
             out = *o;
         }
+        const at::Tensor* m = a[10] == Py_None ? nullptr : tensor(a[10], "mass");
+        if (PyErr_Occurred() || !no_gradients(who, q, c.k, c.v, m, a[11] == Py_None ? nullptr : &out)) return nullptr;
         at::Tensor lse = at::empty({rows, heads}, q->options().dtype(at::kFloat)), scratch;
         t.q = q->data_ptr();
         t.out = out.data_ptr();
@@ -238,9 +252,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         t.lse_row_stride = heads;
         t.rows = rows;
         t.num_heads = static_cast<int32_t>(std::min<int64_t>(heads, INT32_MAX));
-        if (a[10] != Py_None) {
-            const at::Tensor* m = tensor(a[10], "mass");
-            if (!m) return nullptr;
+        if (m) {
             if (m->dim() != 3 || m->scalar_type() != at::kFloat || !m->is_cuda() || m->get_device() != c.index ||
                 m->size(0) != c.kv.num_seqs || m->size(1) != c.kv.kv_heads || (m->size(2) > 1 && m->stride(2) != 1)) {
                 value_error("%s: mass must be [%d, %d, positions] float32 with contiguous rows on the pools' GPU", who,
@@ -277,7 +289,7 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Cache c;
         if (!get_cache(a, &c)) return nullptr;
         const at::Tensor *m = tensor(a[4], "mass"), *dst = tensor(a[5], "dst_table");
-        if (!m || !dst) return nullptr;
+        if (!m || !dst || !no_gradients("kv_evict", m, c.k, c.v)) return nullptr;
         rt_paged_evict_args e = {};
         if (!get_int(a[6], "budget", &e.budget) || !get_int(a[7], "sinks", &e.sinks) || !get_int(a[8], "recent", &e.recent))
             return nullptr;

@@ -22,8 +22,9 @@ sequence b is slot ``j % page_size`` of page ``page_table[b, j // page_size]``.
 ``PagePool`` hands out page numbers; ``PagedKvCache`` keeps pools for several
 layers, the page table and the lengths of a set of sequences, and calls the
 operators.  Wrong types, shapes or devices raise ValueError, failures inside
-the library RtError.  Nothing here is differentiable: the framework trains
-nothing.
+the library RtError.  Nothing here is differentiable, the framework trains
+nothing: tensors that require gradients are refused unless under
+torch.no_grad().
 """
 
 import threading

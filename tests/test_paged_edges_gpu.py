@@ -502,3 +502,34 @@ def test_cache_trims_in_full_pools(spare):
                 assert torch.equal(x[c.page_table[b, j // page].long(), :, j % page], y[dst[b, j // page].long(), :, j % page])
     used = [int(p) for p in c.page_table.flatten() if p >= 0]
     assert sorted(used + c.pool._free) == list(range(c.pool.num_pages))
+
+
+def test_gradients_are_refused_not_dropped():
+    from rich_triplet_b200 import paged
+
+    c = Cache([40, 9], 2, 64, 16, F32, spare=2)
+    kp, vp, table, lens = c.args()
+    q, k = queries(2, 4, 64, F32, 0, False), torch.randn(2, 2, 64, device=DEV)
+    start = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    mass = torch.zeros(2, 2, 50, device=DEV)
+    dst = c.free[:2].view(2, 1).to(DEV)
+
+    def grad(x):
+        return x.detach().clone().requires_grad_()
+
+    calls = [lambda: paged.attend_decode(grad(q), kp, vp, table, lens, scale=0.1),
+             lambda: paged.attend_decode(grad(q) * 2, kp, vp, table, lens, scale=0.1),
+             lambda: paged.attend_decode(q, grad(kp), vp, table, lens, scale=0.1),
+             lambda: paged.attend_decode(q, kp, vp, table, lens, scale=0.1, mass=grad(mass)),
+             lambda: paged.attend_prompt(q, start, 1, kp, grad(vp), table, lens, scale=0.1),
+             lambda: paged.attend_prompt(grad(q), start, 1, kp, vp, table, lens, scale=0.1),
+             lambda: paged.kv_append(kp, vp, grad(k), k, table, lens),
+             lambda: paged.kv_append(kp, vp, k, grad(k), table, lens),
+             lambda: paged.kv_evict(kp, vp, table, lens, grad(mass), dst, budget=8)]
+    for call in calls:
+        refused(ValueError, "not differentiable", call)
+        with torch.no_grad():
+            call()
+        with torch.inference_mode():
+            call()
+    torch.cuda.synchronize()
