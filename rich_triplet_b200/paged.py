@@ -126,6 +126,8 @@ def attend_prompt(q, q_start, max_new, k_pages, v_pages, page_table, lens, *, sc
     sequence b, and each sees the positions up to its own (window, sinks and
     mass as for attend_decode).  ``max_new`` bounds the tokens of a sequence;
     rows beyond it are left as they are.  Returns (out, lse [rows, heads])."""
+    if q_start is None:  # the binding would take it for a decode step
+        raise ValueError("attend_prompt: q_start must be a tensor")
     return _ext.attend(k_pages, v_pages, page_table, lens, q, q_start, max_new, scale, window, sinks, mass, out)
 
 

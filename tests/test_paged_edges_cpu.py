@@ -255,3 +255,13 @@ def test_drop_every_step_costs_the_same_late_in_a_long_sequence():
         c.extend([1] * 8)
         c.drop(1024, 4)
     assert len(seen) <= 2 * 8 * 32 // 8 + 8 and accounted(c)
+
+
+def test_prompt_without_row_starts_is_refused():
+    """Not taken for a decode step, which has none."""
+    from rich_triplet_b200 import paged
+
+    pools = [torch.zeros(4, 2, 16, 64) for _ in range(2)]
+    table, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="q_start must be a tensor"):
+        paged.attend_prompt(torch.zeros(1, 2, 64), None, 1, *pools, table, lens, scale=1.0)
