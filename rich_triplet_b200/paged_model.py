@@ -33,6 +33,8 @@ class PagedGemma3:
 
     def __init__(self, weights: Gemma3Weights, sequences, max_len, page_size=32, dtype=torch.bfloat16, sinks=0,
                  budget=0, recent=64, ctx: Context = None):
+        if budget and not (0 <= sinks and 0 <= recent and sinks + recent <= budget):
+            raise ValueError(f"PagedGemma3: sinks {sinks} + recent {recent} must lie in 0..budget {budget}")
         cfg = self.cfg = weights.cfg
         self.ctx = ctx or Context(0)
         self.stream = torch.cuda.ExternalStream(self.ctx.stream_ptr)
@@ -170,7 +172,8 @@ def main(argv=None):
     a = ap.parse_args(argv)
 
     cfg = Config4.gemma3_4b(vocab_size=262144).with_layers(a.layers)
-    model = PagedGemma3(synth_gemma3(cfg, seed=a.seed), a.seqs, a.prompt + a.steps + 1, sinks=a.sinks, budget=a.budget)
+    model = PagedGemma3(synth_gemma3(cfg, seed=a.seed), a.seqs, a.prompt + a.steps + 1, sinks=a.sinks, budget=a.budget,
+                        recent=max(0, min(64, a.budget - a.sinks)))
     prompts = [list(synth_tokens(a.seed, b, max(1, a.prompt * (b + 1) // a.seqs), cfg.vocab_size)) for b in range(a.seqs)]
     out = [[] for _ in prompts]
     torch.cuda.synchronize()

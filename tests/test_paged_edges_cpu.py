@@ -265,3 +265,16 @@ def test_prompt_without_row_starts_is_refused():
     table, lens = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
     with pytest.raises(ValueError, match="q_start must be a tensor"):
         paged.attend_prompt(torch.zeros(1, 2, 64), None, 1, *pools, table, lens, scale=1.0)
+
+
+def test_model_refuses_budgets_that_no_trim_takes():
+    """Before anything is made, not in the middle of the step that trims first."""
+    from rich_triplet_b200.model import Config4
+    from rich_triplet_b200.paged_model import PagedGemma3
+
+    class Weights:
+        cfg = Config4.tiny()
+
+    for kw in (dict(budget=32), dict(budget=70, sinks=7), dict(budget=-1), dict(budget=64, recent=-1)):
+        with pytest.raises(ValueError, match="must lie in 0..budget"):
+            PagedGemma3(Weights, 1, 64, **kw)
