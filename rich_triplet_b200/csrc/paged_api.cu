@@ -40,6 +40,9 @@ bool strides_ok(int esize, S... s) {
     return ((s >= 0 && s * esize % 16 == 0) && ...);
 }
 
+// The stride of an extent of at most one is never used: its value is `unused`.
+int64_t stride(int64_t extent, int64_t given, int64_t unused) { return extent > 1 ? given : unused; }
+
 constexpr int64_t kMaxPositions = INT32_MAX - 256;  // of a sequence
 
 bool page_size_ok(int page_size) { return page_size >= 8 && page_size <= 256 && (page_size & (page_size - 1)) == 0; }
@@ -94,10 +97,11 @@ int make_kv(rt_ctx* ctx, const char* who, const rt_paged_kv* in, rt::PagedKv* ou
         return fail(ctx, RT_E_SHAPE, "%s: page table of width %d, row stride %lld", who, in->table_width,
                     static_cast<long long>(in->table_stride));
     const int esize = type == rt::kPagedF32 ? 4 : 2;
-    if (!strides_ok(esize, in->page_stride, in->head_stride, in->slot_stride))
+    const int64_t page_stride = stride(in->num_pages, in->page_stride, in->head_dim),
+                  head_stride = stride(in->kv_heads, in->head_stride, in->head_dim);
+    if (!strides_ok(esize, page_stride, head_stride, in->slot_stride))
         return fail(ctx, RT_E_INVAL, "%s: cache strides must be multiples of 16 bytes", who);
-    if (in->slot_stride < in->head_dim || (in->kv_heads > 1 && in->head_stride < in->head_dim) ||
-        (in->num_pages > 1 && in->page_stride < in->head_dim))
+    if (in->slot_stride < in->head_dim || head_stride < in->head_dim || page_stride < in->head_dim)
         return fail(ctx, RT_E_SHAPE, "%s: the rows of the cache overlap", who);
     if (in->num_seqs > 0) {
         if (!in->k || !in->v || !in->lens || (in->table_width > 0 && !in->page_table))
@@ -106,7 +110,7 @@ int make_kv(rt_ctx* ctx, const char* who, const rt_paged_kv* in, rt::PagedKv* ou
     }
     int lg = 3;
     while ((1 << lg) < in->page_size) ++lg;
-    *out = rt::PagedKv{in->k,          in->v,           in->page_stride, in->head_stride, in->slot_stride,
+    *out = rt::PagedKv{in->k,          in->v,           page_stride,     head_stride,     in->slot_stride,
                        in->num_pages,  in->page_table,  in->table_stride, in->lens,       in->table_width,
                        in->num_seqs,   in->kv_heads,    in->head_dim,    lg,              type};
     return RT_OK;
@@ -132,9 +136,11 @@ int make_attn(rt_ctx* ctx, const char* who, const rt_paged_kv* kv, const rt_page
         if (in->rows != kv->num_seqs)
             return fail(ctx, RT_E_SHAPE, "%s: %lld rows for %d sequences", who, static_cast<long long>(in->rows), kv->num_seqs);
     }
+    const int64_t D = kv->head_dim, q_row = stride(in->rows, in->q_row_stride, D), q_head = stride(in->num_heads, in->q_head_stride, D),
+                  out_row = stride(in->rows, in->out_row_stride, D), out_head = stride(in->num_heads, in->out_head_stride, D);
     if (in->rows > 0 && (!in->q || !in->out)) return fail(ctx, RT_E_INVAL, "%s: null q or out", who);
     if (!aligned(in->q) || !aligned(in->out) ||
-        !strides_ok(esize, in->q_row_stride, in->q_head_stride, in->out_row_stride, in->out_head_stride))
+        !strides_ok(esize, q_row, q_head, out_row, out_head))
         return fail(ctx, RT_E_INVAL, "%s: q and out must be 16-byte aligned with strides in multiples of 16 bytes", who);
     if (!apart(in->rows, in->out_row_stride, in->num_heads, in->out_head_stride, kv->head_dim))
         return fail(ctx, RT_E_SHAPE, "%s: the rows of out overlap", who);
@@ -145,7 +151,7 @@ int make_attn(rt_ctx* ctx, const char* who, const rt_paged_kv* kv, const rt_page
         return fail(ctx, RT_E_INVAL, "%s: out overlaps q, which the totals read again", who);
     if (in->mass && !apart(kv->num_seqs, in->mass_seq_stride, kv->kv_heads, in->mass_head_stride, in->mass_cap))
         return fail(ctx, RT_E_SHAPE, "%s: the rows of mass overlap", who);
-    *out = rt::PagedAttn{in->q, in->out, in->q_row_stride, in->q_head_stride, in->out_row_stride, in->out_head_stride,
+    *out = rt::PagedAttn{in->q, in->out, q_row, q_head, out_row, out_head,
                          in->lse, in->lse_row_stride, in->rows, in->num_heads, in->num_heads / kv->kv_heads,
                          in->window, in->sinks, in->max_new, in->scale, in->mass_cap, prompt ? in->q_start : nullptr,
                          in->mass, in->mass_seq_stride, in->mass_head_stride, nullptr};
@@ -230,12 +236,13 @@ int rt_paged_append(rt_ctx* ctx, const rt_paged_kv* in, const rt_paged_rows* r, 
     if (!r->q_start && r->rows != in->num_seqs)
         return fail(ctx, RT_E_SHAPE, "%s: %lld rows for %d sequences", who, static_cast<long long>(r->rows), in->num_seqs);
     if (r->rows == 0 || in->num_seqs == 0) return RT_OK;
+    const int64_t row = stride(r->rows, r->row_stride, in->head_dim), head = stride(in->kv_heads, r->head_stride, in->head_dim);
     if (!r->k || !r->v) return fail(ctx, RT_E_INVAL, "%s: null rows", who);
-    if (!aligned(r->k) || !aligned(r->v) || !strides_ok(st == rt::kPagedF32 ? 4 : 2, r->row_stride, r->head_stride))
+    if (!aligned(r->k) || !aligned(r->v) || !strides_ok(st == rt::kPagedF32 ? 4 : 2, row, head))
         return fail(ctx, RT_E_INVAL, "%s: rows must be 16-byte aligned with strides in multiples of 16 bytes", who);
     DeviceScope scope(ctx->device);
     RT_CHECK_CUDA(ctx, scope.e);
-    const rt::PagedRows a{r->k, r->v, r->row_stride, r->head_stride, r->rows, st, r->q_start};
+    const rt::PagedRows a{r->k, r->v, row, head, r->rows, st, r->q_start};
     RT_CHECK_CUDA(ctx, rt::paged_append_launch(kv, a, stream ? static_cast<cudaStream_t>(stream) : ctx->stream));
     return RT_OK;
 }

@@ -96,6 +96,13 @@ bool int32_rows(const at::Tensor& t, int index, int64_t n) {
     return t.dim() == 1 && t.size(0) == n && t.scalar_type() == at::kInt && t.get_device() == index && t.is_contiguous();
 }
 
+// Whether two tensors of the same sizes have the same strides (those of extents of one say nothing).
+bool same_strides(const at::Tensor& a, const at::Tensor& b) {
+    for (int64_t i = 0; i < a.dim(); ++i)
+        if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+    return true;
+}
+
 struct Cache {
     rt_paged_kv kv;
     const at::Tensor *k, *v;
@@ -108,7 +115,7 @@ bool get_cache(PyObject* const* a, Cache* c) {
     const at::Tensor *k = tensor(a[0], "k_pages"), *v = tensor(a[1], "v_pages"), *table = tensor(a[2], "page_table"),
                      *lens = tensor(a[3], "lens");
     if (!k || !v || !table || !lens) return false;
-    if (k->dim() != 4 || k->sizes() != v->sizes() || k->strides() != v->strides())
+    if (k->dim() != 4 || k->sizes() != v->sizes() || !same_strides(*k, *v))
         return value_error("paged: k_pages and v_pages must be [num_pages, kv_heads, page_size, head_dim] with the same strides");
     c->type = k->scalar_type();
     c->index = k->is_cuda() ? k->get_device() : -1;
@@ -170,7 +177,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!get_cache(a, &c)) return nullptr;
         const at::Tensor *k = tensor(a[4], "k"), *v = tensor(a[5], "v");
         if (!k || !v || !no_gradients("kv_append", k, v, c.k, c.v)) return nullptr;
-        if (k->dim() != 3 || v->sizes() != k->sizes() || v->strides() != k->strides() || k->size(1) != c.kv.kv_heads ||
+        if (k->dim() != 3 || v->sizes() != k->sizes() || !same_strides(*k, *v) || k->size(1) != c.kv.kv_heads ||
             k->size(2) != c.kv.head_dim || k->stride(2) != 1) {
             value_error("kv_append: k and v must be [rows, %d, %d] with the same strides and contiguous rows",
                         c.kv.kv_heads, c.kv.head_dim);

@@ -533,3 +533,37 @@ def test_gradients_are_refused_not_dropped():
         with torch.inference_mode():
             call()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_strides_of_extents_of_one_say_nothing(dtype):
+    """One row, head or page: torch gives its stride any value."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([40], 1, 64, 64, dtype, spare=1)
+    kp, vp = c.kp[c.table[0, :1].long()], c.vp[c.table[0, :1].long()]  # one page
+    table = torch.zeros_like(c.table)
+    q = queries(1, 4, 64, dtype, 0, False)
+    start = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    mass = torch.zeros(2, 1, 1, 40, device=DEV)
+    want = paged.attend_decode(q, kp, vp, table, c.lens_t, scale=0.1, mass=mass[0])
+
+    def odd(x, *strides):
+        return torch.as_strided(x, x.shape, strides)
+
+    kp, vp = odd(kp, 3, 5, 64, 1), odd(vp, 7, 9, 64, 1)
+    for q1, out in ((odd(q, 259, 64, 1), None), (q, odd(torch.zeros_like(q), 1, 64, 1))):
+        got = paged.attend_decode(q1, kp, vp, table, c.lens_t, scale=0.1, out=out)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        got = paged.attend_prompt(q1, start, 1, kp, vp, table, c.lens_t, scale=0.1, mass=mass[1].zero_(), out=out)
+        assert torch.allclose(got[0], want[0], rtol=0.02, atol=0.02) and torch.allclose(mass[1], mass[0], rtol=1e-3)
+    one = odd(q[:, :1], 3, 5, 1)
+    got = paged.attend_decode(one, kp, vp, table, c.lens_t, scale=0.1)
+    assert torch.allclose(got[0], want[0][:, :1], rtol=0.02, atol=0.02)
+    k = torch.randn(1, 1, 64, device=DEV)
+    paged.kv_append(kp, vp, odd(k, 3, 5, 1), odd(k, 2, 1, 1), table, c.lens_t)
+    assert torch.equal(kp[0, 0, 39], k[0, 0].to(dtype)) and torch.equal(vp[0, 0, 39], k[0, 0].to(dtype))
+    # larger extents count
+    c = Cache([40, 9], 2, 64, 16, dtype)
+    q = torch.zeros(2, 259, dtype=dtype, device=DEV)[:, :256].view(2, 4, 64)
+    refused(RtError, "multiples of 16 bytes", paged.attend_decode, q, *c.args(), scale=0.1)
