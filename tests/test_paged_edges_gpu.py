@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from rich_triplet_b200._lib import RtError
-from test_paged_gpu import BF16, DEV, F16, F32, Cache, close, e32, is_visible, queries, reference
+from test_paged_gpu import BF16, DEV, F16, F32, U, Cache, close, e32, is_visible, queries, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -567,3 +567,145 @@ def test_strides_of_extents_of_one_say_nothing(dtype):
     c = Cache([40, 9], 2, 64, 16, dtype)
     q = torch.zeros(2, 259, dtype=dtype, device=DEV)[:, :256].view(2, 4, 64)
     refused(RtError, "multiples of 16 bytes", paged.attend_decode, q, *c.args(), scale=0.1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_graphs_of_every_operator(dtype):
+    """Append, decode and prompt with totals and eviction in one captured graph,
+    replayed with other lengths and rows: the bits of plain calls."""
+    from rich_triplet_b200 import paged
+
+    nkv, d, page = 2, 64, 16
+    c = Cache([300, 64, 200], nkv, d, page, dtype, spare=24)
+    dst = c.free[:24].view(3, 8).to(DEV)
+    q, k = queries(3, 4, d, dtype, 0, False), torch.randn(3, nkv, d, device=DEV)
+    qp = queries(12, 4, d, dtype, 1, False)
+    start = torch.tensor([0, 5, 6, 12], dtype=torch.int32, device=DEV)
+    kp, vp, lens = torch.empty_like(c.kp), torch.empty_like(c.vp), c.lens_t.clone()
+
+    def calls():
+        mass = torch.zeros(3, nkv, 320, device=DEV)
+        paged.kv_append(kp, vp, k, k, c.table, lens)
+        a = paged.attend_decode(q, kp, vp, c.table, lens, scale=0.1, window=150, sinks=3, mass=mass)
+        b = paged.attend_prompt(qp, start, 6, kp, vp, c.table, lens, scale=0.1, mass=mass)
+        e = paged.kv_evict(kp, vp, c.table, lens, mass, dst, budget=120, sinks=3, recent=9)
+        return (*a, *b, mass, *e)
+
+    def fill(n, seed):
+        kp.copy_(c.kp)
+        vp.copy_(c.vp)
+        lens.copy_(torch.tensor(n))
+        g = torch.Generator().manual_seed(seed)
+        q.copy_(torch.randn(q.shape, generator=g))
+        qp.copy_(torch.randn(qp.shape, generator=g))
+        k.copy_(torch.randn(k.shape, generator=g))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        fill([300, 64, 200], 0)
+        calls()
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        got = calls()
+    for n, seed in (([300, 64, 200], 1), ([121, 7, 199], 2), ([290, 60, 6], 3)):
+        fill(n, seed)
+        want = [x.clone() for x in calls()]
+        pools = kp.clone(), vp.clone()
+        fill(n, seed)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for x, y in zip((*got, kp, vp), (*want, *pools)):
+            assert torch.equal(x.nan_to_num(7.0) if x.is_floating_point() else x, y.nan_to_num(7.0) if y.is_floating_point() else y)
+    paged.context(DEV).sync()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 4)])
+def test_tables_and_totals_wider_than_the_lengths(dtype, window, sinks):
+    """Room for 70000 positions a sequence, as a cache that may grow has: outputs,
+    totals and kept positions are those of tables that just fit."""
+    from rich_triplet_b200 import paged
+
+    lens, new, nkv, d, page, wide = [700, 33, 0, 260], [200, 33, 0, 1], 2, 64, 16, 70000
+    c = Cache(lens, nkv, d, page, dtype, spare=4 * 8)
+    table = torch.full((4, wide // page), -1, dtype=torch.int32, device=DEV)
+    table[:, :c.table.shape[1]] = c.table
+    q, qp = queries(4, 4, d, dtype, 0, False), queries(234, 4, d, dtype, 1, False)
+    start = torch.tensor([0, 200, 233, 233, 234], dtype=torch.int32, device=DEV)
+    seen = dict(scale=0.125, window=window, sinks=sinks)
+    dst = c.free[:32].view(4, 8).to(DEV)
+    got = []
+    for t, cap in ((c.table, 700), (table, wide)):
+        mass = torch.zeros(4, nkv, cap, device=DEV)
+        a = paged.attend_decode(q, c.kp, c.vp, t, c.lens_t, mass=mass, **seen)
+        b = paged.attend_prompt(qp, start, 200, c.kp, c.vp, t, c.lens_t, mass=mass, **seen)
+        kept, n, out = paged.kv_evict(c.kp, c.vp, t, c.lens_t, mass, dst, budget=120, sinks=4, recent=30)
+        assert (mass[..., 700:] == 0).all() and (out[..., 120:] == 0).all()
+        got.append((*a, *b, mass[..., :700], kept, n, out[..., :700]))
+    u = U[dtype]
+    for i, (x, y) in enumerate(zip(*got)):
+        if x.dtype == torch.int32:
+            continue
+        # prompts and their totals may be split differently over CTAs: each is within
+        # about u (1 + |value|) of the definition
+        assert torch.equal(torch.isinf(x), torch.isinf(y))
+        fin = torch.isfinite(y)
+        off = (x[fin].double() - y[fin].double()).abs()
+        assert float((off - 4 * u * (1 + y[fin].double().abs())).max() if off.numel() else 0) <= 0, i
+    # the totals decide; equal ones, equal positions
+    mass = got[0][4].contiguous()
+    full = torch.zeros(4, nkv, wide, device=DEV)
+    full[..., :700] = mass
+    a = paged.kv_evict(c.kp, c.vp, c.table, c.lens_t, mass, dst, budget=120, sinks=4, recent=30)
+    b = paged.kv_evict(c.kp, c.vp, table, c.lens_t, full, dst, budget=120, sinks=4, recent=30)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(a[2], b[2][..., :700])
+
+
+@pytest.mark.parametrize("dtype,fmt", [(BF16, 30), (F16, 1), (F32, 0)])
+def test_c_calls_without_lse(dtype, fmt):
+    """rt_paged_prompt and rt_paged_decode with totals and lse NULL: the scratch of
+    rt_paged_scratch stands in, its end untouched; too little of it is refused."""
+    import ctypes
+
+    from rich_triplet_b200 import paged
+    from rich_triplet_b200._lib import lib
+    from test_paged_edges_cpu import Attn, Kv
+
+    nkv, nq, d, page = 2, 4, 64, 16
+    c = Cache([130, 9, 0], nkv, d, page, dtype)
+    start = torch.tensor([0, 40, 49, 49], dtype=torch.int32, device=DEV)
+    scale = 0.125
+    ctx = paged.context(DEV)
+    ctx.sync()
+    kv = Kv(k=c.kp.data_ptr(), v=c.vp.data_ptr(), page_stride=c.kp.stride(0), head_stride=c.kp.stride(1),
+            slot_stride=c.kp.stride(2), num_pages=c.kp.shape[0], fmt=fmt, kv_heads=nkv, head_dim=d, page_size=page,
+            page_table=c.table.data_ptr(), table_stride=c.table.shape[1], table_width=c.table.shape[1], num_seqs=3,
+            lens=c.lens_t.data_ptr())
+    for prompt in (1, 0):
+        rows = 49 if prompt else 3
+        q = queries(rows, nq, d, dtype, prompt, False)
+        want_mass = torch.zeros(3, nkv, 130, device=DEV)
+        if prompt:
+            want, _ = paged.attend_prompt(q, start, 40, *c.args(), scale=scale, mass=want_mass)
+        else:
+            want, _ = paged.attend_decode(q, *c.args(), scale=scale, mass=want_mass)
+        out, mass = torch.empty_like(q), torch.zeros_like(want_mass)
+        a = Attn(q=q.data_ptr(), out=out.data_ptr(), q_row_stride=nq * d, q_head_stride=d, out_row_stride=nq * d,
+                 out_head_stride=d, rows=rows, num_heads=nq, max_new=40, scale=scale, mass_cap=130,
+                 q_start=start.data_ptr() if prompt else None, mass=mass.data_ptr(), mass_seq_stride=nkv * 130,
+                 mass_head_stride=130)
+        need = ctypes.c_uint64()
+        assert lib().rt_paged_scratch(ctypes.byref(kv), ctypes.byref(a), prompt, ctypes.byref(need)) == 0
+        assert need.value >= rows * nq * 4
+        room = torch.full((need.value + 512,), 77, dtype=torch.uint8, device=DEV)
+        torch.cuda.synchronize()
+        call = lib().rt_paged_prompt if prompt else lib().rt_paged_decode
+        a.scratch, a.scratch_bytes = room.data_ptr(), need.value - 1
+        assert call(ctx.h, ctypes.byref(kv), ctypes.byref(a), None) == -1 and "scratch" in ctx.last_error()
+        a.scratch_bytes = need.value
+        assert call(ctx.h, ctypes.byref(kv), ctypes.byref(a), None) == 0, ctx.last_error()
+        ctx.sync()
+        assert torch.equal(out, want) and torch.equal(mass, want_mass) and (room[need.value:] == 77).all()
