@@ -78,11 +78,6 @@ __device__ __forceinline__ void dealloc(uint32_t base, uint32_t cols) {  // one 
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 // a + b on a pair of f32 lanes.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
