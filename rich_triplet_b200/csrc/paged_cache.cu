@@ -119,8 +119,8 @@ __device__ __forceinline__ int block_prefix(int v, int* red, int& total) {
 }
 
 // One CTA per (sequence, KV head).  The keys are read once and stay in
-// registers where the cache holds at most kHeldBlocks blocks (HELD; else each
-// pass reads them again).  Three passes over 11, 11 and 10 bits find the key of
+// registers where a table row has room for at most kHeldBlocks blocks (HELD;
+// else each pass reads them again).  Three passes over 11, 11 and 10 bits find the key of
 // the last position kept, by a histogram in shared memory each; then the kept
 // positions are written in order: a warp owns 256 consecutive positions of a
 // block, so that ballots rank them inside the warp and one prefix over the
@@ -322,7 +322,8 @@ cudaError_t paged_evict_launch(const PagedKv& kv, const PagedEvict& e, cudaStrea
     const dim3 rows(kv.nkv, kv.nseq);
     // A small block's barriers cost less, a large one's threads hold fewer keys
     // each: 700 positions take 7.1 us in 256 threads and 9.2 in 1024, 8192 take
-    // 17.4 and 10.7.
+    // 17.4 and 10.7.  The lengths are on the device, so the room of a table row
+    // decides: short sequences in wide tables run on the larger variants.
     const int64_t cap = static_cast<int64_t>(kv.width) << kv.page_log2;
     if (cap <= 256 * kKeysEach) paged_select_kernel<256, true><<<rows, 256, 0, s>>>(kv, e);
     else if (cap <= kHeldBlocks * 1024 * kKeysEach) paged_select_kernel<1024, true><<<rows, 1024, 0, s>>>(kv, e);

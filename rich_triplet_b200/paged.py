@@ -25,6 +25,11 @@ operators.  Wrong types, shapes or devices raise ValueError, failures inside
 the library RtError.  Nothing here is differentiable, the framework trains
 nothing: tensors that require gradients are refused unless under
 torch.no_grad().
+
+Over f16 and bf16 caches attend_prompt rounds each attention weight to the
+cache's type before it multiplies the values, the sum of the weights being that
+of the unrounded ones; attend_decode multiplies them in two parts.  Scores, sums,
+lse and mass are 32 bits wide everywhere.
 """
 
 import threading
