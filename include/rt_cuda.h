@@ -456,13 +456,14 @@ int rt_qwen35_logits_device(rt_qwen35* eng, const float** out);
  * row (and in an eviction's budget and mass row); pools, queries, outputs and rows
  * 16-byte aligned, all their strides multiples of 16 bytes.
  *
- * Workspace: the context keeps one fixed workspace per stream (by its handle;
- * one per thread for the per-thread default stream), made by the first
- * rt_paged_decode or rt_paged_prompt call on that stream that has rows (make it
- * before a capture: during one it returns RT_E_STATE; append and eviction use no
- * workspace).  It lives until rt_destroy; a graph that captured such calls uses
- * it too, so a replay must not overlap other calls made on the stream it was
- * captured from, and must not run after rt_destroy.
+ * Workspace: the context keeps one fixed workspace per stream (by its handle)
+ * and calling thread, made by the thread's first rt_paged_decode or
+ * rt_paged_prompt call on that stream that has rows (make it before a capture:
+ * during one it returns RT_E_STATE; append and eviction use no workspace).  It
+ * lives until rt_destroy; the next thread takes over those of one that has
+ * ended.  A graph that captured such calls uses it too, so a replay must not
+ * overlap other calls that the thread makes on the stream it was captured from,
+ * and must not run after rt_destroy.
  *
  * Errors of kernels: a prompt kernel whose bounded wait gives up leaves its
  * outputs unwritten and reports to the context; rt_sync returns RT_E_TIMEOUT

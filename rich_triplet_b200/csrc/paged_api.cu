@@ -2,6 +2,10 @@
 // include/rt_cuda.h): argument checks, then the launchers of paged.cuh.
 #include <math.h>
 
+#include <mutex>
+#include <utility>
+#include <vector>
+
 #include "paged.cuh"
 #include "rt_internal.h"
 
@@ -165,11 +169,35 @@ uint64_t scratch_need(const rt::PagedKv& kv, const rt::PagedAttn& a, bool prompt
     return a.rows > INT64_MAX / 8 / a.nq ? UINT64_MAX : (static_cast<uint64_t>(a.rows) * a.nq * 4 + 255) / 256 * 256;
 }
 
-// The stream's workspace, made on first use.
+// A small number of this thread, another thread's once this one has ended.
+int thread_number() {
+    struct Numbers {
+        std::mutex m;
+        std::vector<bool> taken;
+    };
+    static Numbers* const all = new Numbers;  // outlives every thread
+    struct Own {
+        int n = 0;
+        Own() {
+            std::lock_guard<std::mutex> lock(all->m);
+            while (n < static_cast<int>(all->taken.size()) && all->taken[n]) ++n;
+            if (n == static_cast<int>(all->taken.size())) all->taken.push_back(true);
+            else all->taken[n] = true;
+        }
+        ~Own() {
+            std::lock_guard<std::mutex> lock(all->m);
+            all->taken[n] = false;
+        }
+    };
+    static thread_local Own own;
+    return own.n;
+}
+
+// The workspace of this thread's calls on the stream, made on first use.  (Two
+// threads may hold the same stream of a pool without knowing it: a graph that one
+// captured there then shares nothing with the other's calls.)
 int workspace(rt_ctx* ctx, const char* who, cudaStream_t s, void** out) {
-    // the per-thread default stream is another stream in each thread
-    static thread_local char t_own;
-    const void* key = s == cudaStreamPerThread ? static_cast<const void*>(&t_own) : static_cast<const void*>(s);
+    const std::pair<cudaStream_t, int> key(s, thread_number());
     auto it = ctx->paged_ws.find(key);
     if (it != ctx->paged_ws.end()) {
         *out = it->second;

@@ -9,6 +9,7 @@
 #include <map>
 #include <string>
 #include <tuple>
+#include <utility>
 
 #include "../../include/rt_cuda.h"
 #include "gemv.cuh"
@@ -32,8 +33,8 @@ struct rt_ctx {
     // intermediates).
     float* io = nullptr;
     size_t io_floats = 0;
-    // Workspace of the paged-cache calls made on each stream (by its handle).
-    std::map<const void*, void*> paged_ws;
+    // Workspaces of the paged-cache calls, by stream and calling thread.
+    std::map<std::pair<cudaStream_t, int>, void*> paged_ws;
 };
 
 struct rt_w {

@@ -3,7 +3,7 @@
 The operators take torch tensors on the GPU and only enqueue work, on the
 current CUDA stream of the tensors' device, like torch's own operators; the
 context behind them, one per device for all threads of the process, keeps one
-workspace per stream.  They run the rt_paged_* entry points of
+workspace per thread and stream.  They run the rt_paged_* entry points of
 include/rt_cuda.h, whose comments define them; the reference has one
 contiguous cache per layer instead (Gemma3LayerKvCache,
 src/transformer4.rs:1794-1864).

@@ -709,3 +709,40 @@ def test_c_calls_without_lse(dtype, fmt):
         assert call(ctx.h, ctypes.byref(kv), ctypes.byref(a), None) == 0, ctx.last_error()
         ctx.sync()
         assert torch.equal(out, want) and torch.equal(mass, want_mass) and (room[need.value:] == 77).all()
+
+
+def test_a_replay_beside_another_threads_calls_on_the_capture_stream():
+    """Streams come from a pool, so two threads may hold the same one: a graph that
+    the first captured there, replayed elsewhere, meets the second's calls."""
+    from rich_triplet_b200 import paged
+
+    c = Cache([9000, 33], 2, 128, 16, BF16)
+    q = [queries(2, 4, 128, BF16, i, False) for i in range(2)]
+    want = [paged.attend_decode(x, *c.args(), scale=0.1)[0] for x in q]
+    s, elsewhere = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        paged.attend_decode(q[0], *c.args(), scale=0.1)
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out, _ = paged.attend_decode(q[0], *c.args(), scale=0.1)
+    wrong, stop = [], threading.Event()
+
+    def other():
+        with torch.cuda.stream(s):
+            for _ in range(300):
+                if not torch.equal(paged.attend_decode(q[1], *c.args(), scale=0.1)[0], want[1]):
+                    wrong.append("other")
+        stop.set()
+
+    t = threading.Thread(target=other)
+    t.start()
+    with torch.cuda.stream(elsewhere):
+        while not stop.is_set():
+            g.replay()
+            if not torch.equal(out, want[0]):
+                wrong.append("replay")
+    t.join()
+    assert not wrong
+    paged.context(DEV).sync()
