@@ -19,7 +19,8 @@ __global__ void __launch_bounds__(256) paged_decode_mass_kernel(const PagedKv kv
     for (int g = 0; g < a.G; ++g) {
         const int64_t row = static_cast<int64_t>(b) * a.nq + h * a.G + g;
         const float2 nm = wk.norm[row];
-        if (nm.y != 0.f) sum += exp2f(wk.scores[row * wk.score_stride + c] - nm.x) * nm.y;  // 0: no weight at all
+        const float w = exp2f(wk.scores[row * wk.score_stride + c] - nm.x) * nm.y;
+        sum += nm.y != 0.f ? w : 0.f;  // 0: no weight at all
     }
     a.mass[b * a.mass_seq + h * a.mass_head + j] += sum;
 }
