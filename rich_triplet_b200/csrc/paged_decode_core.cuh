@@ -33,8 +33,8 @@
 //
 // Measured (B200): one sequence of 131071 positions, 8 heads on 4 of 256, bf16:
 // 95 us, 5.6 TB/s (the SMs finish between 62 and 84 us, the join of 74 parts
-// takes 8).  64 sequences, 1.05 GB of f32: 190 us,
-// 5.5 TB/s.  64 windows of 1028: 46 us, 5.8 TB/s.  301 positions: 9.2 us, six
+// takes 8).  64 sequences, 1.05 GB of f32: 194 us, 5.4 TB/s (205 to 212 in a row of
+// calls).  64 windows of 1028: 45 us, 5.8 TB/s.  301 positions: 9.0 us, six
 // dependent trips to memory (length, page, rows, part, counter, parts).
 //
 // A state has seen no weight where its sum is 0, whatever its maximum: NaN scores

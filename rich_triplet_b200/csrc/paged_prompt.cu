@@ -38,8 +38,9 @@
 // kErrMbarTimeout, waits (bounded) for its copies and products in flight,
 // frees its tensor memory and returns.
 //
-// Measured (B200): 8192 tokens, 32 heads on 16 of 128, all visible: 610 us,
-// 900 TFLOP/s.  There a pair of 128 x 128 tiles takes 3800 clocks where its
+// Measured (B200): 8192 tokens, 32 heads on 16 of 128, all visible: 640 to 660 us
+// in a row of calls, 850 TFLOP/s (615 us where it runs a few times only).  There
+// a pair of 128 x 128 tiles takes 3800 clocks where its
 // products take 2050: the chain scores -> weights (2000) -> product with V ->
 // next scores of a tile is only half hidden behind the other tile's.  6185
 // tokens in windows of 1024, 16 heads on 4 of 256: 167 us; a 128 x 128 tile
