@@ -465,9 +465,9 @@ int rt_qwen35_logits_device(rt_qwen35* eng, const float** out);
  * overlap other calls that the thread makes on the stream it was captured from,
  * and must not run after rt_destroy.
  *
- * Errors of kernels: a prompt kernel whose bounded wait gives up leaves its
- * outputs unwritten and reports to the context; rt_sync returns RT_E_TIMEOUT
- * then.  rt_sync waits for the context's own stream only: synchronise the
+ * Errors of kernels: a prompt kernel whose bounded wait gives up reports to the
+ * context, and rt_sync returns RT_E_TIMEOUT; the call's outputs and totals mean
+ * nothing then.  rt_sync waits for the context's own stream only: synchronise the
  * streams of the calls first. */
 typedef struct {
     void *k, *v;                                   /* pools */
